@@ -431,6 +431,144 @@ int pk_set_sampling_fast_sums(pk_engine *e, int on);
 int pk_sampler_state(pk_engine *e, uint64_t *rng, int32_t *history_host, int cap,
                      int *history_len);
 
+/* ── paged KV caches: several requests of different lengths ──
+ * picchio decodes one sequence and pk_decode_batch steps its sequences in
+ * lockstep over caches of a fixed size; these serve requests that come, grow
+ * and end one by one, over a pool of pages that they share (no reference
+ * counterpart). A step: pk_plan_pages hands out pages and gives every new row
+ * its position and slot, pk_store_pages rotates the rows and fills the slots,
+ * pk_attention_paged attends over the pages; pk_attention_packed attends over
+ * prompts that need no cache. The calls take device pointers and plain
+ * numbers only, synchronise nothing and can be captured; what depends on the
+ * requests' lengths is read on the device, so that a captured step serves
+ * later lengths too. */
+
+/* Element types of activations and caches. */
+#define PK_T_F32  0
+#define PK_T_F16  1
+#define PK_T_BF16 2
+
+/* One layer's paged keys and values: [n_pages][n_kv_heads][page_size][head_dim]
+ * each. Slot s is row s % page_size of page s / page_size. page_size a power
+ * of two from 8 to 256, head_dim a multiple of 16 up to 128, n_pages *
+ * page_size below 2^31, both pointers 16-byte aligned. */
+typedef struct pk_pages {
+    void *k_dev, *v_dev;
+    int32_t type;              /* PK_T_*                                    */
+    int32_t n_pages, page_size, n_kv_heads, head_dim;
+} pk_pages;
+
+/* Free pages are kept in a ring of n_pages entries: ring_state_dev[0] is the
+ * place of the first, [1] their number (at the start: 0 and n_pages, the ring
+ * holding every page id once), [2] and [3] the library's (0 at the start).
+ * For request r with lengths old_len_dev[r] and new_len_dev[r] in positions
+ * (cut to 0 .. max_blocks * page_size), in order of r:
+ *  - a request that grows gets ceil(new / page_size) - ceil(old / page_size)
+ *    pages from the ring's front, in order, into its row of table_dev, and new
+ *    - old rows. A request whose pages or rows, added to those of all growing
+ *    requests before it (served or not), exceed the ring's pages or max_tokens
+ *    gets nothing and keeps its old length;
+ *  - a request that shrinks gives the pages behind its new length back to the
+ *    ring's end, in order, and their table entries become -1. Pages given back
+ *    in this call are handed out by later ones.
+ * Results: len_dev[r] the length reached; cu_q_dev[r] .. cu_q_dev[r + 1] the
+ * request's rows (cu_q_dev[n_req] rows in all); for row t pos_dev[t] its
+ * position and slot_dev[t] its slot (-1 where the table names no page); for the
+ * rows from cu_q_dev[n_req] to max_tokens position 0 and slot -1. A table entry
+ * below ceil(old / page_size) has to be a page that the request holds. n_req
+ * up to 4096; the old and new lengths may not overlap len_dev. */
+typedef struct pk_page_plan {
+    int32_t n_req, max_blocks, n_pages, page_size, max_tokens;
+    const int32_t *old_len_dev, *new_len_dev;    /* [n_req]                  */
+    int32_t *table_dev;                          /* [n_req][max_blocks]      */
+    int32_t *ring_dev, *ring_state_dev;          /* [n_pages], [4]           */
+    int32_t *len_dev, *cu_q_dev;                 /* [n_req], [n_req + 1]     */
+    int32_t *slot_dev, *pos_dev;                 /* [max_tokens]             */
+} pk_page_plan;
+int pk_plan_pages(pk_engine *e, const pk_page_plan *p);
+
+/* Rows t of a step: q_out[t] = the query heads of q[t], and the key heads of
+ * k[t] into the K pages at slot_dev[t], both rotated by the angles of position
+ * pos_dev[t] (element j with j + head_dim / 2, the cosines and sines of
+ * rope_dev[pos][j], as gqa_attention rotates, picchio.c:431-466; rope_dev null:
+ * not rotated), and the value heads of v[t] into the V pages. The arithmetic is
+ * fp32, rounded once to the type of the activations or of the pages. A row
+ * whose slot is not in 0 .. n_pages * page_size - 1, or whose position is not in
+ * 0 .. rope_len - 1 while rope_dev is set, is left out: nothing of it is
+ * written. The slots of the rows that are not left out differ from each other.
+ * Row t of q, k, v and q_out starts t * stride elements behind the pointer, its
+ * heads side by side; pointers 16-byte aligned, strides multiples of 8. q_out
+ * may be q; the other buffers may not overlap. The activations are of type
+ * `type`, and the pages of the same type or, with PK_T_F32, of any. n_heads 0:
+ * no queries (q_dev and q_out_dev are not read). */
+typedef struct pk_kv_rows {
+    int32_t n_tokens, n_heads, type, rope_len;
+    const void *q_dev, *k_dev, *v_dev;
+    void *q_out_dev;
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    const int32_t *pos_dev, *slot_dev;           /* [n_tokens]               */
+    const float *rope_dev;                       /* [rope_len][head_dim / 2][2] */
+    pk_pages pages;
+} pk_kv_rows;
+int pk_store_pages(pk_engine *e, const pk_kv_rows *r);
+
+/* The engine's own table for rope_dev (YaRN, picchio.c:431-466): [*n_pos]
+ * positions of the configuration's head_dim. */
+const float *pk_engine_rope(pk_engine *e, int *n_pos);
+
+/* Causal attention of n_seq whole prompts packed row behind row: rows
+ * cu_dev[s] .. cu_dev[s + 1] are prompt s (cu_dev[0] >= 0, ascending, at most
+ * n_tokens; what is beyond is cut). Row i sees the rows of its own prompt up to
+ * itself, with window > 0 the last `window` of them. n_heads query heads share
+ * n_kv_heads key / value heads in equal groups. scale 0: 1 / sqrt(head_dim).
+ * sinks_dev (optional): a logit per query head that joins the softmax without
+ * a value (gqa_attention's sinks, picchio.c:504-623). lse_dev (optional):
+ * [n_tokens][n_heads] the logarithm of the softmax's denominator, sink
+ * included. Rows of no prompt are left as they were. Scores, softmax and sums
+ * are fp32; with 16-bit types the probabilities are rounded to that type for the
+ * product with V, with PK_T_F32 products are exact to about 2^-23. Row t of q,
+ * k, v and out starts t * stride elements behind the pointer, its heads side by
+ * side; pointers 16-byte aligned, strides multiples of 8, head_dim a multiple
+ * of 16 up to 128; out may not overlap the inputs. max_len: a bound on the
+ * prompts' lengths; rows beyond it are not computed. */
+typedef struct pk_attn_packed {
+    int32_t type, n_heads, n_kv_heads, head_dim;
+    int32_t n_tokens, n_seq, max_len, window;
+    float scale;
+    const void *q_dev, *k_dev, *v_dev;
+    void *out_dev;
+    int64_t q_stride, k_stride, v_stride, out_stride;
+    const int32_t *cu_dev;                       /* [n_seq + 1]              */
+    const float *sinks_dev;                      /* [n_heads] or null        */
+    float *lse_dev;                              /* [n_tokens][n_heads] or null */
+} pk_attn_packed;
+int pk_attention_packed(pk_engine *e, const pk_attn_packed *a);
+
+/* Attention of new rows over paged caches: rows cu_q_dev[r] .. cu_q_dev[r + 1]
+ * are the last rows of request r, whose kv_len_dev[r] positions (its new rows
+ * among them, stored before the call) lie on the pages of its row of table_dev.
+ * Row i of request r is at position kv_len - (its rows) + i and sees the
+ * positions up to its own, with window > 0 the last `window` of them. A position
+ * on a table entry outside 0 .. n_pages - 1 is not seen; a row that sees
+ * nothing is 0 (lse: its sink, or -infinity). kv_len is cut to 0 .. max_blocks *
+ * page_size. max_q: a bound on a request's rows (rows beyond it are not
+ * computed); max_kv: the host's bound on the lengths, which only chooses the
+ * launch (0: max_blocks * page_size). The pages have the queries' type or, with
+ * PK_T_F32, any. The rest as in pk_attention_packed. */
+typedef struct pk_attn_paged {
+    int32_t type, n_heads, n_tokens, n_req, max_blocks, max_q, max_kv, window;
+    float scale;
+    const void *q_dev;
+    void *out_dev;
+    int64_t q_stride, out_stride;
+    const int32_t *cu_q_dev, *kv_len_dev;        /* [n_req + 1], [n_req]     */
+    const int32_t *table_dev;                    /* [n_req][max_blocks]      */
+    const float *sinks_dev;                      /* [n_heads] or null        */
+    float *lse_dev;                              /* [n_tokens][n_heads] or null */
+    pk_pages pages;
+} pk_attn_paged;
+int pk_attention_paged(pk_engine *e, const pk_attn_paged *a);
+
 /* ── measurement (no reference counterpart: benchmark plumbing) ──
  * With profiling on, the engine brackets each launch of the listed kernels
  * with a pair of HIP events on its stream; pk_engine_profile_read syncs and

@@ -16,6 +16,7 @@ PK_OK = 0
 ERRORS = {-1: "PK_ERR_ARG", -2: "PK_ERR_HIP", -3: "PK_ERR_OOM", -4: "PK_ERR_UNSUPPORTED",
           -5: "PK_ERR_MISSING", -6: "PK_ERR_CONTEXT_FULL"}
 FMT_F32, FMT_INT8, FMT_INT4 = 0, 1, 2
+T_F32, T_F16, T_BF16 = 0, 1, 2
 PROF_EXPERT_GATE_UP, PROF_EXPERT_DOWN, PROF_ROUTER, PROF_COMBINE = 0, 1, 2, 3
 PROF_MOE_FFN, PROF_LM_HEAD, PROF_ATTENTION = 4, 5, 6
 
@@ -54,6 +55,156 @@ class PkLayerHost(C.Structure):
                 ("wq", PkQtHost), ("wk", PkQtHost), ("wv", PkQtHost), ("wo", PkQtHost),
                 ("bq", C.c_void_p), ("bk", C.c_void_p), ("bv", C.c_void_p), ("bo", C.c_void_p),
                 ("sinks", C.c_void_p), ("router", C.c_void_p), ("router_bias", C.c_void_p)]
+
+
+class PkPages(C.Structure):
+    """pk_pages: one layer's paged keys and values."""
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("type", C.c_int32), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class PkPagePlan(C.Structure):
+    _fields_ = [("n_req", C.c_int32), ("max_blocks", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+                ("max_tokens", C.c_int32), ("old_len_dev", C.c_void_p), ("new_len_dev", C.c_void_p),
+                ("table_dev", C.c_void_p), ("ring_dev", C.c_void_p), ("ring_state_dev", C.c_void_p),
+                ("len_dev", C.c_void_p), ("cu_q_dev", C.c_void_p), ("slot_dev", C.c_void_p), ("pos_dev", C.c_void_p)]
+
+
+class PkKvRows(C.Structure):
+    _fields_ = [("n_tokens", C.c_int32), ("n_heads", C.c_int32), ("type", C.c_int32), ("rope_len", C.c_int32),
+                ("q_dev", C.c_void_p), ("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("q_out_dev", C.c_void_p),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_out_stride", C.c_int64),
+                ("pos_dev", C.c_void_p), ("slot_dev", C.c_void_p), ("rope_dev", C.c_void_p), ("pages", PkPages)]
+
+
+class PkAttnPacked(C.Structure):
+    _fields_ = [("type", C.c_int32), ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("n_tokens", C.c_int32), ("n_seq", C.c_int32), ("max_len", C.c_int32), ("window", C.c_int32),
+                ("scale", C.c_float), ("q_dev", C.c_void_p), ("k_dev", C.c_void_p), ("v_dev", C.c_void_p),
+                ("out_dev", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("out_stride", C.c_int64), ("cu_dev", C.c_void_p), ("sinks_dev", C.c_void_p), ("lse_dev", C.c_void_p)]
+
+
+class PkAttnPaged(C.Structure):
+    _fields_ = [("type", C.c_int32), ("n_heads", C.c_int32), ("n_tokens", C.c_int32), ("n_req", C.c_int32),
+                ("max_blocks", C.c_int32), ("max_q", C.c_int32), ("max_kv", C.c_int32), ("window", C.c_int32),
+                ("scale", C.c_float), ("q_dev", C.c_void_p), ("out_dev", C.c_void_p), ("q_stride", C.c_int64),
+                ("out_stride", C.c_int64), ("cu_q_dev", C.c_void_p), ("kv_len_dev", C.c_void_p),
+                ("table_dev", C.c_void_p), ("sinks_dev", C.c_void_p), ("lse_dev", C.c_void_p), ("pages", PkPages)]
+
+
+# Argument records of the paged-cache operators from device tensors. A record
+# holds its tensors alive and may be used for any number of calls (the lengths,
+# tables and rows are read on the device at each call).
+
+def _type(t):
+    import torch
+    try:
+        return {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16}[t.dtype]
+    except KeyError:
+        raise ValueError(f"element type {t.dtype} (float32, float16 or bfloat16)") from None
+
+
+def _ids(t, shape, what):
+    import torch
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous int32 tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _floats(t, shape, what):
+    import torch
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous float32 tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _rows(t, shape, dtype, what):
+    """(address, row stride) of [rows, heads, head_dim], a row's heads side by side."""
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or (t.numel() and
+                                                              (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]))):
+        raise ValueError(f"{what}: rows of shape {tuple(shape)} and type {dtype}, each row's heads side by side; got "
+                         f"{t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _one_device(*ts):
+    ds = {t.device for t in ts if t is not None}
+    if len(ds) > 1:
+        raise ValueError(f"tensors on several devices: {sorted(map(str, ds))}")
+
+
+def pages(k, v):
+    """pk_pages of K and V page tensors [n_pages, n_kv_heads, page_size, head_dim]."""
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or not (k.is_contiguous() and v.is_contiguous()):
+        raise ValueError("pages: two contiguous tensors [n_pages, n_kv_heads, page_size, head_dim] of one type")
+    _one_device(k, v)
+    p = PkPages(k.data_ptr(), v.data_ptr(), _type(k), k.shape[0], k.shape[2], k.shape[1], k.shape[3])
+    p.keep = (k, v)
+    return p
+
+
+def page_plan(old_len, new_len, table, ring, state, page_size, length, cu_q, slot, pos):
+    """pk_page_plan: lengths [n], table [n, max_blocks], ring [n_pages], state [4];
+    results length [n], cu_q [n + 1], slot and pos [max_tokens]."""
+    n = old_len.shape[0]
+    _one_device(old_len, new_len, table, ring, state, length, cu_q, slot, pos)
+    p = PkPagePlan(n, table.shape[1], ring.shape[0], page_size, slot.shape[0], _ids(old_len, (n,), "old_len"),
+                   _ids(new_len, (n,), "new_len"), _ids(table, (n, table.shape[1]), "table"),
+                   _ids(ring, (ring.shape[0],), "ring"), _ids(state, (4,), "state"), _ids(length, (n,), "length"),
+                   _ids(cu_q, (n + 1,), "cu_q"), _ids(slot, (slot.shape[0],), "slot"), _ids(pos, (slot.shape[0],), "pos"))
+    p.keep = (old_len, new_len, table, ring, state, length, cu_q, slot, pos)
+    return p
+
+
+def kv_rows(q, k, v, q_out, pos, slot, pages, rope=None):
+    """pk_kv_rows: q and q_out [T, n_heads, head_dim] (both None: no queries), k
+    and v [T, n_kv_heads, head_dim]; rope None, a table [positions, head_dim / 2,
+    2], or Engine.rope() for the engine's own."""
+    T, kvh, hd = k.shape[0], pages.n_kv_heads, pages.head_dim
+    table, rope = (rope, None) if isinstance(rope, tuple) else (None, rope)
+    _one_device(q, k, v, q_out, pos, slot, rope, pages.keep[0])
+    H = 0 if q is None else q.shape[1]
+    (qp, qs), (op, os_) = ((None, 0), (None, 0)) if q is None else (_rows(q, (T, H, hd), k.dtype, "q"),
+                                                                    _rows(q_out, (T, H, hd), k.dtype, "q_out"))
+    (kp, ks), (vp, vs) = _rows(k, (T, kvh, hd), k.dtype, "k"), _rows(v, (T, kvh, hd), k.dtype, "v")
+    n = 0 if rope is None else rope.shape[0]
+    address, n = table or (_floats(rope, (n, hd // 2, 2), "rope"), n)
+    r = PkKvRows(T, H, _type(k), n, qp, kp, vp, op, qs, ks, vs, os_, _ids(pos, (T,), "pos"), _ids(slot, (T,), "slot"),
+                 address, pages)
+    r.keep = (q, k, v, q_out, pos, slot, pages.keep, rope)
+    return r
+
+
+def attn_packed(q, k, v, out, cu, max_len, window=0, scale=0.0, sinks=None, lse=None):
+    """pk_attn_packed: q and out [T, n_heads, head_dim], k and v [T, n_kv_heads,
+    head_dim], cu [prompts + 1]."""
+    T, H, hd = q.shape
+    kvh = k.shape[1]
+    _one_device(q, k, v, out, cu, sinks, lse)
+    (qp, qs), (op, os_) = _rows(q, (T, H, hd), q.dtype, "q"), _rows(out, (T, H, hd), q.dtype, "out")
+    (kp, ks), (vp, vs) = _rows(k, (T, kvh, hd), q.dtype, "k"), _rows(v, (T, kvh, hd), q.dtype, "v")
+    a = PkAttnPacked(_type(q), H, kvh, hd, T, cu.shape[0] - 1, max_len, window, scale, qp, kp, vp, op, qs, ks, vs, os_,
+                     _ids(cu, (cu.shape[0],), "cu"), _floats(sinks, (H,), "sinks"), _floats(lse, (T, H), "lse"))
+    a.keep = (q, k, v, out, cu, sinks, lse)
+    return a
+
+
+def attn_paged(q, out, cu_q, kv_len, table, pages, max_q, max_kv=0, window=0, scale=0.0, sinks=None, lse=None):
+    """pk_attn_paged: q and out [T, n_heads, head_dim], cu_q [n + 1], kv_len [n],
+    table [n, max_blocks]."""
+    T, H, hd = q.shape
+    n = kv_len.shape[0]
+    _one_device(q, out, cu_q, kv_len, table, sinks, lse, pages.keep[0])
+    (qp, qs), (op, os_) = _rows(q, (T, H, pages.head_dim), q.dtype, "q"), _rows(out, (T, H, hd), q.dtype, "out")
+    a = PkAttnPaged(_type(q), H, T, n, table.shape[1], max_q, max_kv, window, scale, qp, op, qs, os_,
+                    _ids(cu_q, (n + 1,), "cu_q"), _ids(kv_len, (n,), "kv_len"),
+                    _ids(table, (n, table.shape[1]), "table"), _floats(sinks, (H,), "sinks"),
+                    _floats(lse, (T, H), "lse"), pages)
+    a.keep = (q, out, cu_q, kv_len, table, sinks, lse, pages.keep)
+    return a
 
 
 def gptoss_cfg(**kw):
@@ -154,6 +305,11 @@ def lib():
         "pk_forward_token": (C.c_int, [vp, C.c_int, C.c_int, vp, vp]),
         "pk_prefill_tokens": (C.c_int, [vp, vp, C.c_int, C.c_int, vp]),
         "pk_generate": (C.c_int, [vp, vp, C.c_int, C.c_int, vp]),
+        "pk_plan_pages": (C.c_int, [vp, C.POINTER(PkPagePlan)]),
+        "pk_store_pages": (C.c_int, [vp, C.POINTER(PkKvRows)]),
+        "pk_engine_rope": (vp, [vp, C.POINTER(C.c_int)]),
+        "pk_attention_packed": (C.c_int, [vp, C.POINTER(PkAttnPacked)]),
+        "pk_attention_paged": (C.c_int, [vp, C.POINTER(PkAttnPaged)]),
         "pk_engine_profile": (C.c_int, [vp, C.c_int]),
         "pk_engine_profile_read": (C.c_int, [vp, C.c_int, C.POINTER(C.c_double), C.POINTER(i64)]),
         "pk_engine_stall": (C.c_int, [vp, C.c_int]),
@@ -468,6 +624,37 @@ class Engine:
         out = np.empty(n_steps, np.int32)
         check(self.L.pk_decode_replay(self.h, tok, pos, n_steps, ptr(out)))
         return out
+
+    # paged caches: the records of page_plan, kv_rows, attn_packed, attn_paged
+    def _own_device(self, rec):
+        if rec.keep[1].device != self.device:
+            raise ValueError(f"tensors on {rec.keep[1].device}, engine on {self.device}")
+
+    def plan_pages(self, plan):
+        """Pages, row starts, slots and positions of a step (pk_plan_pages)."""
+        self._own_device(plan)
+        check(self.L.pk_plan_pages(self.h, plan))
+
+    def store_pages(self, rows):
+        """A step's rows rotated, their keys and values into the pages (pk_store_pages)."""
+        self._own_device(rows)
+        check(self.L.pk_store_pages(self.h, rows))
+
+    def rope(self):
+        """(address, positions) of the engine's rotation table (pk_engine_rope)."""
+        n = C.c_int()
+        p = self.L.pk_engine_rope(self.h, C.byref(n))
+        return p, n.value
+
+    def attention_packed(self, a):
+        """Causal attention of packed prompts (pk_attention_packed)."""
+        self._own_device(a)
+        check(self.L.pk_attention_packed(self.h, a))
+
+    def attention_paged(self, a):
+        """Attention of new rows over paged caches (pk_attention_paged)."""
+        self._own_device(a)
+        check(self.L.pk_attention_paged(self.h, a))
 
     def expert_apply(self, layer, eid, x_dev, dst_dev, w):
         check(self.L.pk_expert_apply(self.h, layer, eid, ptr(x_dev), ptr(dst_dev), w))
