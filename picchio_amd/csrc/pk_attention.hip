@@ -1,47 +1,14 @@
 // pk_attention.hip — attention of packed prompts (pk_attention_packed) and of
-// new rows over paged caches (pk_attention_paged).
-//
-// Row i of a request at position p sees the positions j in (p - window, p]:
-// s_j = scale q . k_j, m = max(max_j s_j, sink), l = sum_j exp(s_j - m) +
-// exp(sink - m), o = sum_j exp(s_j - m) v_j / l, lse = m + ln l. One pass over
-// the positions carries the running m, l and o, rescaled where m grows.
-#include "pk_engine.h"
-#include "pk_types.h"
+// new rows over paged caches (pk_attention_paged): the calls' checks and the
+// choice of kernel.
+#include "pk_attention.h"
 
 #include <math.h>
 
 namespace {
 
-// What both calls hand to a kernel: the requests' rows of q, and where their
-// positions' keys and values lie (rows of k and v, or pages).
-struct attn_args {
-    const void *q, *k, *v;
-    void *out;
-    int64_t q_stride, k_stride, v_stride, out_stride;
-    const int32_t *cu, *kv_len, *table;          // kv_len, table: null for packed prompts
-    const float *sinks;
-    float *lse;
-    int n_tokens, n_req, max_q, window;
-    int H, KVH, hd;
-    int n_pages, page_shift, max_blocks;
-    float scale;
-};
-
-// Request r's first row, number of rows and of positions, within the buffers
-// whatever cu and kv_len hold.
-struct span {
-    int row0, rows, kv;
-};
-__device__ __forceinline__ span request(const attn_args &a, int r) {
-    span s;
-    s.row0 = min(max(a.cu[r], 0), a.n_tokens);
-    s.rows = max(min(max(a.cu[r + 1], 0), a.n_tokens) - s.row0, 0);
-    s.kv = a.kv_len ? min(max(a.kv_len[r], 0), a.max_blocks << a.page_shift) : s.rows;
-    return s;
-}
-
 template <typename A, typename C, bool PAGED>
-__global__ __launch_bounds__(64) void k_attn_rows(attn_args a) {
+__global__ __launch_bounds__(64) void k_attn_rows(pk_attn_args a) {
     const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, hd = a.hd;
     const int kvh = h / (a.H / a.KVH);
     int lo = 0, hi = a.n_req - 1;
@@ -50,7 +17,7 @@ __global__ __launch_bounds__(64) void k_attn_rows(attn_args a) {
         if (a.cu[mid] <= t) lo = mid;
         else hi = mid - 1;
     }
-    const span s = request(a, lo);
+    const pk_span s = pk_request(a, lo);
     const int i = t - s.row0;
     if (i < 0 || i >= s.rows || i >= a.max_q) return;
     const int p = s.kv - s.rows + i;
@@ -58,7 +25,7 @@ __global__ __launch_bounds__(64) void k_attn_rows(attn_args a) {
     __shared__ float q[128];
     for (int c = lane; c < hd; c += 64) q[c] = (float)((const A *)a.q)[(int64_t)t * a.q_stride + h * hd + c];
     __syncthreads();
-    const float c2 = a.scale * 1.4426950408889634f;
+    const float c2 = a.scale2;
     float m = a.sinks ? a.sinks[h] * 1.4426950408889634f : -INFINITY, l = a.sinks ? 1.0f : 0.0f, o0 = 0.0f, o1 = 0.0f;
     for (int j0 = first; j0 <= p; j0 += 64) {
         const int j = j0 + lane;
@@ -114,6 +81,24 @@ int check_common(const pk_engine *e, int H, int KVH, int hd, int n_tokens, int n
 
 }  // namespace
 
+int pk_attn_workspace(pk_engine *e, int64_t floats, int64_t counts) {
+    if (floats <= e->att_ws_floats && counts <= e->att_ws_counts) return PK_OK;
+    PK_CHECK(!e->capturing, PK_ERR_ARG, "attention: the workspace would grow while capturing; run the call once before");
+    floats = std::max(floats, e->att_ws_floats);
+    counts = std::max(counts, e->att_ws_counts);
+    const pk_buf_bytes b[] = {{(void **)&e->att_ws, floats * 4}, {(void **)&e->att_cnt, counts * 4}};
+    const int rc = pk_regrow(e, e->att_use, b, 2);
+    if (rc != PK_OK) {                                       // (the old ones are kept for a graph, or are gone)
+        if (!e->att_ws || !e->att_cnt) e->att_ws_floats = e->att_ws_counts = 0;
+        return rc;
+    }
+    e->att_ws_floats = e->att_ws_counts = 0;
+    PK_HIP(hipMemsetAsync(e->att_cnt, 0, (size_t)counts * 4, e->stream));
+    e->att_ws_floats = floats;
+    e->att_ws_counts = counts;
+    return PK_OK;
+}
+
 extern "C" int pk_attention_packed(pk_engine *e, const pk_attn_packed *p) {
     PK_CHECK(e && p, PK_ERR_ARG, "null argument");
     PK_CHECK(pk_type_size(p->type), PK_ERR_ARG, "type %d", p->type);
@@ -124,13 +109,14 @@ extern "C" int pk_attention_packed(pk_engine *e, const pk_attn_packed *p) {
     PK_TRY(pk_check_rows(p->k_dev, p->k_stride, p->n_kv_heads, p->head_dim, "k"));
     PK_TRY(pk_check_rows(p->v_dev, p->v_stride, p->n_kv_heads, p->head_dim, "v"));
     PK_TRY(pk_check_rows(p->out_dev, p->out_stride, p->n_heads, p->head_dim, "out"));
-    attn_args a{};
+    pk_attn_args a{};
     a.q = p->q_dev, a.k = p->k_dev, a.v = p->v_dev, a.out = p->out_dev;
     a.q_stride = p->q_stride, a.k_stride = p->k_stride, a.v_stride = p->v_stride, a.out_stride = p->out_stride;
     a.cu = p->cu_dev, a.sinks = p->sinks_dev, a.lse = p->lse_dev;
     a.n_tokens = p->n_tokens, a.n_req = p->n_seq, a.max_q = p->max_len, a.window = p->window;
     a.H = p->n_heads, a.KVH = p->n_kv_heads, a.hd = p->head_dim;
-    a.scale = p->scale > 0.0f ? p->scale : 1.0f / sqrtf((float)p->head_dim);
+    a.scale2 = (p->scale > 0.0f ? p->scale : 1.0f / sqrtf((float)p->head_dim)) * PK_LOG2E;
+    a.type = a.cache_type = p->type;
     pk_device_scope dev(e->device);
     PK_TRY(dev.rc);
     const dim3 grid((unsigned)a.n_tokens, (unsigned)a.H);
@@ -152,16 +138,20 @@ extern "C" int pk_attention_paged(pk_engine *e, const pk_attn_paged *p) {
     PK_CHECK(p->cu_q_dev && p->kv_len_dev && p->table_dev, PK_ERR_ARG, "attention_paged: null argument");
     PK_TRY(pk_check_rows(p->q_dev, p->q_stride, p->n_heads, g.head_dim, "q"));
     PK_TRY(pk_check_rows(p->out_dev, p->out_stride, p->n_heads, g.head_dim, "out"));
-    attn_args a{};
+    pk_attn_args a{};
     a.q = p->q_dev, a.k = g.k_dev, a.v = g.v_dev, a.out = p->out_dev;
     a.q_stride = p->q_stride, a.out_stride = p->out_stride;
     a.cu = p->cu_q_dev, a.kv_len = p->kv_len_dev, a.table = p->table_dev, a.sinks = p->sinks_dev, a.lse = p->lse_dev;
     a.n_tokens = p->n_tokens, a.n_req = p->n_req, a.max_q = p->max_q, a.window = p->window;
     a.H = p->n_heads, a.KVH = g.n_kv_heads, a.hd = g.head_dim;
     a.n_pages = g.n_pages, a.page_shift = __builtin_ctz((unsigned)g.page_size), a.max_blocks = p->max_blocks;
-    a.scale = p->scale > 0.0f ? p->scale : 1.0f / sqrtf((float)g.head_dim);
+    a.scale2 = (p->scale > 0.0f ? p->scale : 1.0f / sqrtf((float)g.head_dim)) * PK_LOG2E;
+    a.type = p->type, a.cache_type = g.type;
     pk_device_scope dev(e->device);
     PK_TRY(dev.rc);
+    const int64_t cap = (int64_t)p->max_blocks * g.page_size;
+    const int max_kv = (int)(p->max_kv > 0 ? std::min<int64_t>(p->max_kv, cap) : cap);
+    if ((int64_t)a.max_q * (a.H / a.KVH) <= PK_FEW_ROWS) return pk_launch_attn_few(e, a, max_kv);
     const dim3 grid((unsigned)a.n_tokens, (unsigned)a.H);
 #define PK_ATTN(A, C) k_attn_rows<A, C, true><<<grid, 64, 0, e->stream>>>(a)
     PK_BY_TYPES(p->type, g.type, PK_ATTN);

@@ -112,10 +112,11 @@ struct pk_engine {
     uint64_t *att_t = nullptr;                // k_attn_oproj hand-over words: [heads x head_dim]
 
     bool capturing = false;                  // inside pk_capture_begin/end
-    // One token per set of growing buffers (b_*, g_*): a captured graph
+    // One token per set of growing buffers (b_*, g_*, att_ws): a captured graph
     // (pk_graph), whose kernels may address the buffers, shares the tokens of its
     // time. Buffers outgrown meanwhile stay until no graph holds their token.
-    std::shared_ptr<char> b_use = std::make_shared<char>(), g_use = std::make_shared<char>();
+    std::shared_ptr<char> b_use = std::make_shared<char>(), g_use = std::make_shared<char>(),
+                          att_use = std::make_shared<char>();
     struct outgrown_set {
         std::shared_ptr<char> use;
         std::vector<void *> bufs;
@@ -186,6 +187,11 @@ struct pk_engine {
     // default), false = exact int8 limbs (PK_GROUPED_F16 / pk_set_grouped_f16)
     bool grouped_f16 = true;
     int32_t *g_exps = nullptr, *g_pairs = nullptr, *g_tiles = nullptr;
+    // paged and packed attention (pk_attention.hip): the parts of rows whose
+    // positions are split over workgroups, and their arrival counters
+    int64_t att_ws_floats = 0, att_ws_counts = 0;
+    float *att_ws = nullptr;
+    uint32_t *att_cnt = nullptr;
     // sampler (pk_sample.hip): device state, host mirror of its parameters,
     // kept entries (value, index) for vocabularies up to samp_cap entries
     pk_sampler_dev *samp = nullptr;

@@ -184,7 +184,7 @@ static void engine_free(pk_engine *e) {
                     e->b_eo, e->b_sel, e->b_perm, e->p_H, e->p_XN, e->p_qkv, e->p_att,
                     e->p_part, e->p_ids, e->bd_logits, e->bd_toks, e->g_limbs, e->g_exps, e->g_pairs, e->g_tiles,
                     e->lm_bval, e->lm_bidx, e->dstate, e->step_out, e->samp, e->samp_av, e->samp_ai, e->samp_ws, e->hn_q, e->act_q, e->b_xq, e->b_actq, e->b_pairs, e->b_tiles,
-                    e->moe_act_t, e->moe_eo_t, e->moe_cont_t, e->att_t, e->skinny_ws, e->lm_t};
+                    e->moe_act_t, e->moe_eo_t, e->moe_cont_t, e->att_t, e->skinny_ws, e->lm_t, e->att_ws, e->att_cnt};
     for (void *p : ptrs) pk_dev_free(e, p);
     for (auto &o : e->outgrown)
         for (void *p : o.bufs) pk_dev_free(e, p);
@@ -543,7 +543,7 @@ extern "C" int pk_engine_stall(pk_engine *e, int usec) {
 struct pk_graph {
     hipGraph_t graph = nullptr;
     hipGraphExec_t exec = nullptr;
-    std::shared_ptr<char> uses[2];            // the engine's buffers' tokens at the capture (pk_regrow)
+    std::shared_ptr<char> uses[3];            // the engine's buffers' tokens at the capture (pk_regrow)
 };
 
 extern "C" int pk_capture_begin(pk_engine *e) {
@@ -571,6 +571,7 @@ extern "C" int pk_capture_end(pk_engine *e, pk_graph **out) {
     }
     g->uses[0] = e->b_use;
     g->uses[1] = e->g_use;
+    g->uses[2] = e->att_use;
     *out = g;
     return PK_OK;
 }
