@@ -13,7 +13,8 @@ OUT = os.path.join(HERE, "libpicchio_hip.so")
 OBJ = os.path.join(HERE, "_build")
 SOURCES = ["pk_i4.hip", "pk_i4_rows.hip", "pk_moe.hip", "pk_dense.hip", "pk_engine.hip", "pk_decode.hip",
            "pk_prefill.hip", "pk_mfma.hip", "pk_sample.hip", "pk_exact.hip",
-           "pk_paged.hip", "pk_attention.hip", "pk_attn_few.hip", "pk_container.cpp"]
+           "pk_paged.hip", "pk_attention.hip", "pk_attn_few.hip", "pk_attn_tile.hip",
+           "pk_container.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -ffp-contract=off: every fused multiply-add in the kernels is an explicit

@@ -23,6 +23,7 @@ struct pk_attn_args {
     const float *sinks;
     float *lse;
     int n_tokens, n_req, max_q, window;
+    int few_only;                                // requests of more than max_q rows: left to another launch
     int H, KVH, hd;
     int n_pages, page_shift, max_blocks;
     float scale2;                                // scale * log2 e
@@ -52,6 +53,8 @@ int pk_attn_workspace(pk_engine *e, int64_t floats, int64_t counts);
 // holds; the launchers.
 constexpr int PK_FEW_ROWS = 32;
 int pk_launch_attn_few(pk_engine *e, const pk_attn_args &a, int max_kv);
+// Requests with more than `cut` of these (the rest is k_attn_few's).
+int pk_launch_attn_tile(pk_engine *e, const pk_attn_args &a, int cut, int max_kv);
 
 // ───────── moves between the lanes of a wave ─────────
 // Maximum and sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48: a 32 x 32 or 16 x 16

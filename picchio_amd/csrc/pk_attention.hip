@@ -7,67 +7,6 @@
 
 namespace {
 
-template <typename A, typename C, bool PAGED>
-__global__ __launch_bounds__(64) void k_attn_rows(pk_attn_args a) {
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, hd = a.hd;
-    const int kvh = h / (a.H / a.KVH);
-    int lo = 0, hi = a.n_req - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (a.cu[mid] <= t) lo = mid;
-        else hi = mid - 1;
-    }
-    const pk_span s = pk_request(a, lo);
-    const int i = t - s.row0;
-    if (i < 0 || i >= s.rows || i >= a.max_q) return;
-    const int p = s.kv - s.rows + i;
-    const int first = a.window > 0 ? max(p - a.window + 1, 0) : 0;
-    __shared__ float q[128];
-    for (int c = lane; c < hd; c += 64) q[c] = (float)((const A *)a.q)[(int64_t)t * a.q_stride + h * hd + c];
-    __syncthreads();
-    const float c2 = a.scale2;
-    float m = a.sinks ? a.sinks[h] * 1.4426950408889634f : -INFINITY, l = a.sinks ? 1.0f : 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int j0 = first; j0 <= p; j0 += 64) {
-        const int j = j0 + lane;
-        int64_t at = -1;
-        int64_t vat = -1;
-        if (j <= p) {
-            if (PAGED) {
-                const int page = a.table[(int64_t)lo * a.max_blocks + (j >> a.page_shift)];
-                if (page >= 0 && page < a.n_pages)
-                    at = vat = ((((int64_t)page * a.KVH + kvh) << a.page_shift) + (j & ((1 << a.page_shift) - 1))) * hd;
-            } else {
-                at = (int64_t)(s.row0 + j) * a.k_stride + kvh * hd;
-                vat = (int64_t)(s.row0 + j) * a.v_stride + kvh * hd;
-            }
-        }
-        float sc = -INFINITY;
-        if (at >= 0) {
-            sc = 0.0f;
-            for (int c = 0; c < hd; ++c) sc = __builtin_fmaf(q[c], (float)((const C *)a.k)[at + c], sc);
-            sc *= c2;
-        }
-        const float mn = fmaxf(m, pk_wave_max_f(sc));
-        if (mn == -INFINITY) continue;
-        const float r = exp2f(m - mn), pr = at >= 0 ? exp2f(sc - mn) : 0.0f;
-        l = l * r + pk_wave_sum_f(pr);
-        o0 *= r, o1 *= r;
-        for (int k = 0; k < 64; ++k) {
-            const int64_t b = __shfl(vat, k);
-            const float w = __shfl(pr, k);
-            if (b < 0) continue;
-            if (lane < hd) o0 = __builtin_fmaf(w, (float)((const C *)a.v)[b + lane], o0);
-            if (lane + 64 < hd) o1 = __builtin_fmaf(w, (float)((const C *)a.v)[b + lane + 64], o1);
-        }
-        m = mn;
-    }
-    const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-    A *dst = (A *)a.out + (int64_t)t * a.out_stride + h * hd;
-    if (lane < hd) dst[lane] = (A)(o0 * inv);
-    if (lane + 64 < hd) dst[lane + 64] = (A)(o1 * inv);
-    if (a.lse && lane == 0) a.lse[(int64_t)t * a.H + h] = m * 0.6931471805599453f + logf(l);
-}
-
 int check_common(const pk_engine *e, int H, int KVH, int hd, int n_tokens, int n_req, int max_q, int window, float scale) {
     PK_CHECK(n_tokens >= 0 && n_req >= 0 && max_q >= 0 && window >= 0, PK_ERR_ARG,
              "attention: %d rows, %d requests of up to %d rows, window %d", n_tokens, n_req, max_q, window);
@@ -119,12 +58,7 @@ extern "C" int pk_attention_packed(pk_engine *e, const pk_attn_packed *p) {
     a.type = a.cache_type = p->type;
     pk_device_scope dev(e->device);
     PK_TRY(dev.rc);
-    const dim3 grid((unsigned)a.n_tokens, (unsigned)a.H);
-    if (p->type == PK_T_F32) k_attn_rows<float, float, false><<<grid, 64, 0, e->stream>>>(a);
-    else if (p->type == PK_T_F16) k_attn_rows<pk_f16, pk_f16, false><<<grid, 64, 0, e->stream>>>(a);
-    else k_attn_rows<pk_bf16, pk_bf16, false><<<grid, 64, 0, e->stream>>>(a);
-    PK_HIP(hipGetLastError());
-    return PK_OK;
+    return pk_launch_attn_tile(e, a, 0, p->max_len);
 }
 
 extern "C" int pk_attention_paged(pk_engine *e, const pk_attn_paged *p) {
@@ -151,11 +85,17 @@ extern "C" int pk_attention_paged(pk_engine *e, const pk_attn_paged *p) {
     PK_TRY(dev.rc);
     const int64_t cap = (int64_t)p->max_blocks * g.page_size;
     const int max_kv = (int)(p->max_kv > 0 ? std::min<int64_t>(p->max_kv, cap) : cap);
-    if ((int64_t)a.max_q * (a.H / a.KVH) <= PK_FEW_ROWS) return pk_launch_attn_few(e, a, max_kv);
-    const dim3 grid((unsigned)a.n_tokens, (unsigned)a.H);
-#define PK_ATTN(A, C) k_attn_rows<A, C, true><<<grid, 64, 0, e->stream>>>(a)
-    PK_BY_TYPES(p->type, g.type, PK_ATTN);
-#undef PK_ATTN
-    PK_HIP(hipGetLastError());
-    return PK_OK;
+    // Few rows of every request: k_attn_few, bound by the reads of K and V. Else the
+    // requests with few rows there (a tile of 128 or 256 columns would be
+    // mostly empty for them), the others in tiles.
+    const int G = a.H / a.KVH;
+    if ((int64_t)a.max_q * G <= PK_FEW_ROWS) return pk_launch_attn_few(e, a, max_kv);
+    int cut = 0;
+    if (a.n_req > 1 && G <= PK_FEW_ROWS) {
+        cut = G <= 16 ? 16 : PK_FEW_ROWS;
+        pk_attn_args few = a;
+        few.max_q = cut / G, few.few_only = 1;
+        PK_TRY(pk_launch_attn_few(e, few, max_kv));
+    }
+    return pk_launch_attn_tile(e, a, cut, max_kv);
 }

@@ -56,7 +56,7 @@ __device__ __forceinline__ seg few_seg(const pk_attn_args &a, int r) {
     g.s = pk_request(a, r);
     const int p0 = max(g.s.kv - g.s.rows, 0);                  // the first row's position
     g.first = a.window > 0 ? max(p0 - a.window + 1, 0) & ~(KT - 1) : 0;
-    g.tiles = g.s.rows ? max((g.s.kv - g.first + KT - 1) / KT, 1) : 0;
+    g.tiles = g.s.rows && !(a.few_only && g.s.rows > a.max_q) ? max((g.s.kv - g.first + KT - 1) / KT, 1) : 0;
     return g;
 }
 

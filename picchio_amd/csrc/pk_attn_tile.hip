@@ -1,0 +1,528 @@
+// pk_attn_tile.hip — attention of many rows: packed prompts, and chunks of new
+// rows over paged caches.
+//
+// A workgroup takes BM columns: rows of one request times the query heads of
+// one KV head, rows first, so that BM / G neighbouring rows share every key
+// and value it reads and a window or the causal edge costs few tiles. Its four waves hold 32
+// MQ columns each and go over the keys in tiles of KT, staged through LDS: S^T = K Q^T,
+// then O^T = V^T P^T. A lane of a 32 x 32 product holds one query's scores of
+// 4 keys out of 8, in the order in which the second product may take them, so
+// that probabilities stay in registers; V comes out of LDS transposed
+// (ds_read_b64_tr_b16). Rows of LDS are XOR-swizzled in 16-byte pieces against
+// bank conflicts.
+//
+// fp32 activations run on the bf16 products as well: a value is three bf16 (its 24
+// bits, 8 at a time, exactly), and of the nine partial products the six above
+// 2^-24 of the result are taken, each exact, summed in fp32. A bf16 cache needs
+// three of them, an fp16 cache five. That is 6 x 16 cycles against 256 of the fp32
+// instructions. Not finite values would meet zeros among the partial
+// products; so such values of V are left out of the product and added one by
+// one, and a key with one makes the rows that see it NaN.
+//
+// Where the columns are too few for the device, the keys are split too: each
+// part leaves m, l and o, and k_attn_join adds them up in order.
+#include "pk_attention.h"
+
+namespace {
+
+constexpr int TILE_THREADS = 256, TILE_WAVES = 4;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T, int N>
+struct regs {
+    typedef T type __attribute__((ext_vector_type(N)));
+};
+
+__device__ __forceinline__ f32x16 mfma(pk_f16x8 a, pk_f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma(pk_bf16x8 a, pk_bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ bool not_finite(T v) {
+    return !(__builtin_fabsf((float)v) <= 3.4028234e38f);
+}
+
+// A value's planes: itself in T, or N bf16 that add up to it.
+template <typename T, int N, typename V8>
+__device__ __forceinline__ void planes(const V8 &x, typename regs<T, 8>::type (&p)[N]) {
+    if constexpr (N == 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[0][i] = (T)x[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float v = (float)x[i];
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const uint32_t hi = __float_as_uint(v) & 0xffff0000u;
+                p[n][i] = __builtin_bit_cast(T, (uint16_t)(hi >> 16));
+                v = v - __uint_as_float(hi);
+            }
+        }
+    }
+}
+
+// Which columns a workgroup has.
+struct place {
+    pk_span s;
+    int r, tile, tiles;      // request, its tile and number of tiles; r < 0: none
+    int idx0, n_idx;         // first column, number of columns of the request
+    int p_lo, p_hi;          // positions of the first and last row
+    int first, n_t;          // first key, tiles of keys
+};
+// Request r's tiles are numbered from floor(row0 G / BM) + r on: at least as many
+// numbers as it has tiles, known without the other requests' lengths.
+template <int BM, int KT>
+__device__ __forceinline__ place find(const pk_attn_args &a, int64_t b, int cut, int *found) {
+    const int G = a.H / a.KVH;
+    if (threadIdx.x == 0) *found = -1;
+    __syncthreads();
+    for (int r = threadIdx.x; r < a.n_req; r += blockDim.x) {
+        const int64_t x = min(max(a.cu[r], 0), a.n_tokens), y = min(max(a.cu[r + 1], 0), a.n_tokens);
+        if (x * G / BM + r <= b && b < y * G / BM + r + 1) *found = r;
+    }
+    __syncthreads();
+    place p;
+    p.r = *found;
+    if (p.r < 0) return p;
+    p.s = pk_request(a, p.r);
+    p.n_idx = min(p.s.rows, a.max_q) * G;
+    p.tiles = (p.n_idx + BM - 1) / BM;
+    const int64_t j = b - ((int64_t)p.s.row0 * G / BM + p.r);
+    if (j < 0 || j >= p.tiles || p.n_idx <= cut) {
+        p.r = -1;
+        return p;
+    }
+    p.tile = p.tiles - 1 - (int)j;                       // the ones with the most keys first
+    p.idx0 = p.tile * BM;
+    const int before = p.s.kv - p.s.rows;
+    p.p_lo = before + p.idx0 / G;
+    p.p_hi = before + (min(p.idx0 + BM, p.n_idx) - 1) / G;
+    p.first = a.window > 0 ? max(p.p_lo - a.window + 1, 0) & ~(KT - 1) : 0;
+    p.n_t = max(p.p_hi + 1 - p.first + KT - 1, 0) / KT;
+    return p;
+}
+
+template <typename A>
+__device__ __forceinline__ void store4(A *dst, float x, float y, float z, float w) {
+    typename regs<A, 4>::type v;
+    v[0] = (A)x, v[1] = (A)y, v[2] = (A)z, v[3] = (A)w;
+    *reinterpret_cast<typename regs<A, 4>::type *>(dst) = v;
+}
+
+constexpr int tile_keys(int hdp, int kp) { return hdp <= 64 || kp == 1 ? 64 : 32; }
+
+template <typename T, typename A, typename C, int HDP, int MQ, int QP, int KP, bool PAGED>
+__global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, int cut, int splits, float *part) {
+    constexpr int KT = tile_keys(HDP, KP), BM = 32 * MQ * TILE_WAVES;
+    constexpr int NB = KT / 32, QS = HDP / 16, HT = HDP / 32, US = KT / 16;
+    constexpr int CPR = HDP / 8, RPP = TILE_THREADS / CPR, NP = KT / RPP, ROWB = HDP * 2;
+    constexpr bool PLANES = QP > 1;
+    typedef typename regs<T, 8>::type t8;
+    typedef typename regs<C, 8>::type c8;
+    typedef typename regs<A, 8>::type a8;
+
+    __shared__ __attribute__((aligned(16))) uint8_t sK[KP][KT * ROWB], sV[KP][KT * ROWB];
+    __shared__ unsigned long long odd_keys[2];
+    __shared__ int found;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, c32 = lane & 31;
+    const int kvh = blockIdx.x % a.KVH, G = a.H / a.KVH, hd = a.hd;
+    const int64_t slot = blockIdx.x / a.KVH;
+    const place pl = find<BM, KT>(a, slot, cut, &found);
+    if (pl.r < 0) return;
+    const int t_first = (int)((int64_t)pl.n_t * blockIdx.y / splits), t_end = (int)((int64_t)pl.n_t * (blockIdx.y + 1) / splits);
+    const int before = pl.s.kv - pl.s.rows, end = pl.p_hi + 1;
+    const int32_t *tab = PAGED ? a.table + (int64_t)pl.r * a.max_blocks : nullptr;
+    const int ps = PAGED ? 1 << a.page_shift : 0;
+
+    // ── queries ──
+    t8 q[MQ][QP][QS];
+    int pos[MQ];
+    const int w0 = pl.idx0 + wave * 32 * MQ;                    // the wave's first column
+    const bool active = w0 < pl.n_idx;
+    const int w_lo = before + w0 / G, w_hi = before + (min(w0 + 32 * MQ, pl.n_idx) - 1) / G;
+#pragma unroll
+    for (int m = 0; m < MQ; ++m) {
+        const int idx = w0 + m * 32 + c32, i = idx / G;
+        const bool on = idx < pl.n_idx;
+        pos[m] = on ? before + i : w_hi;
+        const A *src = (const A *)a.q + (int64_t)(pl.s.row0 + i) * a.q_stride + ((int64_t)kvh * G + (idx - i * G)) * hd;
+#pragma unroll
+        for (int s = 0; s < QS; ++s) {
+            const int e = 16 * s + 8 * h;
+            a8 x = {};
+            if (on && e < hd) x = *reinterpret_cast<const a8 *>(src + e);
+            t8 p[QP];
+            planes<T, QP>(x, p);
+#pragma unroll
+            for (int n = 0; n < QP; ++n) q[m][n][s] = p[n];
+        }
+    }
+
+    f32x16 o[MQ][HT];
+    float mx[MQ], ls[MQ];
+#pragma unroll
+    for (int m = 0; m < MQ; ++m) {
+        mx[m] = -INFINITY;
+        ls[m] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < HT; ++x)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[m][x][i] = 0.0f;
+    }
+
+    // ── staging: this thread's pieces of a tile's keys and values ──
+    const int my_key = tid / CPR, my_c = tid % CPR;
+    c8 rk[NP], rv[NP];
+    const auto look = [&](int t, uint64_t &ok) {
+        const int j = pl.first + t * KT + (lane & (KT - 1));
+        int pg = 0;
+        bool good = j < end;
+        if constexpr (PAGED) {
+            pg = tab[min(j, max(end - 1, 0)) >> a.page_shift];
+            good = good && pg >= 0 && pg < a.n_pages;
+            pg = good ? pg : 0;
+        }
+        ok = __ballot(good);
+        return pg;
+    };
+    const auto load = [&](int t, int pgs) {
+        const int base = pl.first + t * KT, e = my_c * 8 < hd ? my_c * 8 : 0;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const int kk = n * RPP + my_key, j = base + kk;
+            int64_t ak, av;
+            if constexpr (PAGED) {
+                const int pg = __shfl(pgs, kk);
+                ak = av = ((((int64_t)pg * a.KVH + kvh) << a.page_shift) + (j & (ps - 1))) * hd + e;
+            } else {
+                const int64_t row = pl.s.row0 + min(j, end - 1);
+                ak = row * a.k_stride + kvh * hd + e;
+                av = row * a.v_stride + kvh * hd + e;
+            }
+            rk[n] = *reinterpret_cast<const c8 *>((const C *)a.k + ak);
+            rv[n] = *reinterpret_cast<const c8 *>((const C *)a.v + av);
+        }
+    };
+    uint64_t ok = 0, ok_next = 0;
+    int pgs_next = 0;
+    if (t_first < t_end) {
+        const int pgs = look(t_first, ok);
+        load(t_first, pgs);
+        if (t_first + 1 < t_end) pgs_next = look(t_first + 1, ok_next);
+    }
+    if (tid < 2) odd_keys[tid] = 0;
+
+    for (int t = t_first; t < t_end; ++t) {
+        const int base = pl.first + t * KT;
+        const uint64_t all = KT == 64 ? ~0ull : (1ull << KT) - 1, ok_now = ok & all;
+        // a tile that some row of the workgroup does not see whole
+        const bool edge = ok_now != all || base + KT - 1 > pl.p_lo || (a.window > 0 && base <= pl.p_hi - a.window);
+        __syncthreads();                                        // the previous tile has been read
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const int kk = n * RPP + my_key;
+            if (!(ok_now >> kk & 1) || my_c * 8 >= hd) rk[n] = c8{}, rv[n] = c8{};
+            if (edge || PLANES) {
+                // values that are not finite and that some rows do not see (with
+                // planes: any): left out here, added one by one below
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) bad |= not_finite(rv[n][i]);
+                if (bad) {
+                    const int j = base + kk;
+                    if (PLANES || j > pl.p_lo || (a.window > 0 && j <= pl.p_hi - a.window)) atomicOr(&odd_keys[t & 1], 1ull << kk);
+                }
+            }
+            t8 pk[KP], pv[KP];
+            planes<T, KP>(rk[n], pk);
+            planes<T, KP>(rv[n], pv);
+#pragma unroll
+            for (int x = 0; x < KP; ++x) {
+                *reinterpret_cast<t8 *>(&sK[x][kk * ROWB + ((my_c ^ (kk & 7)) << 4)]) = pk[x];
+                *reinterpret_cast<t8 *>(&sV[x][kk * ROWB + ((my_c ^ ((kk & 3) << 1)) << 4)]) = pv[x];
+            }
+        }
+        __syncthreads();
+        uint64_t odd = 0;
+        if (edge || PLANES) {
+            odd = odd_keys[t & 1];
+            if (odd) {                                          // (rare) their rows of V: zero
+                __syncthreads();
+                for (uint64_t left = odd; left; left &= left - 1) {
+                    const int kk = __ffsll((unsigned long long)left) - 1;
+                    for (int x = tid; x < KP * CPR; x += TILE_THREADS)
+                        *reinterpret_cast<t8 *>(&sV[x / CPR][kk * ROWB + ((x % CPR) << 4)]) = t8{};
+                }
+                __syncthreads();
+            }
+        }
+        if (tid == 0) odd_keys[(t + 1) & 1] = 0;
+        if (t + 1 < t_end) {
+            load(t + 1, pgs_next);
+            ok = ok_next;
+            if (t + 2 < t_end) pgs_next = look(t + 2, ok_next);
+        }
+        // a tile that the wave's rows do not see at all
+        if (!active || base > w_hi || (a.window > 0 && base + KT - 1 <= w_lo - a.window)) continue;
+
+        // ── S^T = K Q^T ──
+        f32x16 s[MQ][NB];
+#pragma unroll
+        for (int m = 0; m < MQ; ++m)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[m][b][i] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < QS; ++x)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int kp = 0; kp < KP; ++kp) {
+                    const int kk = b * 32 + c32;
+                    const t8 kf = *reinterpret_cast<const t8 *>(&sK[kp][kk * ROWB + (((2 * x + h) ^ (kk & 7)) << 4)]);
+#pragma unroll
+                    for (int qp = 0; qp < QP && qp + kp < 3; ++qp)
+#pragma unroll
+                        for (int m = 0; m < MQ; ++m) s[m][b] = mfma(kf, q[m][qp][x], s[m][b]);
+                }
+        const bool masked = ok_now != all || base + KT - 1 > w_lo || (a.window > 0 && base <= w_hi - a.window);
+        if (masked) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int kk = b * 32 + 8 * (i >> 2) + 4 * h + (i & 3), j = base + kk;
+                    const bool there = ok_now >> kk & 1;
+#pragma unroll
+                    for (int m = 0; m < MQ; ++m)
+                        if (!(there && j <= pos[m] && (a.window <= 0 || j > pos[m] - a.window))) s[m][b][i] = -INFINITY;
+                }
+        }
+        // ── probabilities ──
+        t8 p[MQ][QP][US];
+#pragma unroll
+        for (int m = 0; m < MQ; ++m) {
+            float top = s[m][0][0];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[m][b][i]);
+            {
+                const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * a.scale2;
+            }
+            // the reference only moves when a score is 2^8 above it: what
+            // lies between makes sums and probabilities no less exact
+            if (__any(top > mx[m] + 8.0f)) {
+                const float mn = fmaxf(mx[m], top), ref = mn == -INFINITY ? 0.0f : mn, f = __builtin_amdgcn_exp2f(mx[m] - ref);
+                mx[m] = mn;
+                ls[m] *= f;
+#pragma unroll
+                for (int x = 0; x < HT; ++x) o[m][x] *= f;
+            }
+            const float ref = mx[m] == -INFINITY ? 0.0f : mx[m];
+            float sum = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[m][b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][b][i], a.scale2, -ref));
+                    sum += s[m][b][i];
+                }
+            ls[m] += sum;
+#pragma unroll
+            for (int u = 0; u < US; ++u) {
+                typename regs<float, 8>::type x;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = s[m][u >> 1][8 * (u & 1) + i];
+                t8 pp[QP];
+                planes<T, QP>(x, pp);
+#pragma unroll
+                for (int n = 0; n < QP; ++n) p[m][n][u] = pp[n];
+            }
+        }
+        // ── O^T += V^T P^T: the keys of step u in the order of the scores' registers ──
+        {
+            const int kr = 4 * h + ((lane & 15) >> 2), c0 = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), sub = (lane & 1) << 3;
+            const int sw = (kr & 3) << 1;
+#pragma unroll
+            for (int u = 0; u < US; ++u)
+#pragma unroll
+                for (int x = 0; x < HT; ++x)
+#pragma unroll
+                    for (int kp = 0; kp < KP; ++kp) {
+                        const int at = (16 * u + kr) * ROWB + (((4 * x + c0) ^ sw) << 4) + sub;
+                        typedef __attribute__((address_space(3))) s16x4 lds4;
+                        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)&sV[kp][at]);
+                        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)&sV[kp][at + 8 * ROWB]);
+                        typename regs<short, 8>::type vv;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) vv[i] = v0[i], vv[4 + i] = v1[i];
+                        const t8 vf = __builtin_bit_cast(t8, vv);
+#pragma unroll
+                        for (int qp = 0; qp < QP && qp + kp < 3; ++qp)
+#pragma unroll
+                            for (int m = 0; m < MQ; ++m) o[m][x] = mfma(vf, p[m][qp][u], o[m][x]);
+                    }
+        }
+        // ── values that are not finite, on the rows that see them ──
+        while (odd) {
+            const int kk = __ffsll((unsigned long long)odd) - 1, j = base + kk;
+            odd &= odd - 1;
+            int64_t at;
+            if constexpr (PAGED) at = ((((int64_t)tab[j >> a.page_shift] * a.KVH + kvh) << a.page_shift) + (j & (ps - 1))) * hd;
+            else at = (int64_t)(pl.s.row0 + j) * a.v_stride + kvh * hd;
+            const C *src = (const C *)a.v + at;
+#pragma unroll
+            for (int m = 0; m < MQ; ++m) {
+                float pr = 0.0f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (b == kk >> 5 && i == 4 * ((kk & 31) >> 3) + (kk & 3)) pr = s[m][b][i];
+                pr = __shfl(pr, c32 + 32 * ((kk >> 2) & 1));
+                if (j <= pos[m] && (a.window <= 0 || j > pos[m] - a.window))
+#pragma unroll
+                    for (int x = 0; x < HT; ++x)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int e = 32 * x + 8 * (i >> 2) + 4 * h + (i & 3);
+                            if (e < hd) o[m][x][i] = __builtin_fmaf(pr, (float)src[e], o[m][x][i]);
+                        }
+            }
+        }
+    }
+
+    // ── out ──
+#pragma unroll
+    for (int m = 0; m < MQ; ++m) {
+        const int col = wave * 32 * MQ + m * 32 + c32, idx = pl.idx0 + col;
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(ls[m]), __float_as_uint(ls[m]), false, false);
+        float l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+        if (idx >= pl.n_idx) continue;
+        if (splits == 1) {
+            const int i = idx / G, hq = kvh * G + (idx - i * G);
+            const int64_t row = pl.s.row0 + i;
+            float ref = mx[m] == -INFINITY ? 0.0f : mx[m], f = 1.0f;
+            if (a.sinks) {
+                const float sk = a.sinks[hq] * PK_LOG2E, top = fmaxf(mx[m], sk), to = top == -INFINITY ? 0.0f : top;
+                f = __builtin_amdgcn_exp2f(mx[m] - to);
+                l = __builtin_fmaf(l, f, __builtin_amdgcn_exp2f(sk - to));
+                ref = to;
+            }
+            const float inv = l == 0.0f ? 0.0f : f / l;
+            A *dst = (A *)a.out + row * a.out_stride + (int64_t)hq * hd;
+#pragma unroll
+            for (int x = 0; x < HT; ++x)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const int e = 32 * x + 8 * y + 4 * h;
+                    if (e < hd)
+                        store4(dst + e, o[m][x][4 * y] * inv, o[m][x][4 * y + 1] * inv, o[m][x][4 * y + 2] * inv,
+                               o[m][x][4 * y + 3] * inv);
+                }
+            if (a.lse && h == 0) a.lse[row * a.H + hq] = l == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * PK_LN2;
+        } else {
+            float *dst = part + ((slot * a.KVH + kvh) * splits + blockIdx.y) * (BM * (HDP + 2));
+            if (h == 0) dst[col] = mx[m], dst[BM + col] = l;
+            if (t_first < t_end)
+#pragma unroll
+                for (int x = 0; x < HT; ++x)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const int e = 32 * x + 8 * y + 4 * h;
+                        if (e < hd)
+                            store4(dst + 2 * BM + (int64_t)col * HDP + e, o[m][x][4 * y], o[m][x][4 * y + 1], o[m][x][4 * y + 2],
+                                   o[m][x][4 * y + 3]);
+                    }
+        }
+    }
+}
+
+// The parts of split keys, added up in order: four elements of a column per thread.
+template <typename A, int BM, int HDP, int KT>
+__global__ __launch_bounds__(TILE_THREADS) void k_attn_join(pk_attn_args a, int cut, int splits, const float *__restrict__ part) {
+    __shared__ int found;
+    const int kvh = blockIdx.x % a.KVH, G = a.H / a.KVH, quads = a.hd >> 2;
+    const int64_t slot = blockIdx.x / a.KVH;
+    const place pl = find<BM, KT>(a, slot, cut, &found);
+    if (pl.r < 0) return;
+    const float *src = part + (slot * a.KVH + kvh) * splits * (BM * (HDP + 2));
+    const int cols = min(BM, pl.n_idx - pl.idx0);
+    for (int x = blockIdx.y * TILE_THREADS + threadIdx.x; x < cols * quads; x += gridDim.y * TILE_THREADS) {
+        const int col = x / quads, e = (x - col * quads) * 4, idx = pl.idx0 + col, i = idx / G, hq = kvh * G + (idx - i * G);
+        const float sk = a.sinks ? a.sinks[hq] * PK_LOG2E : -INFINITY;
+        float top = sk;
+        for (int y = 0; y < splits; ++y) top = fmaxf(top, src[(int64_t)y * (BM * (HDP + 2)) + col]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float l = __builtin_amdgcn_exp2f(sk - ref);
+        f32x4 acc = {0, 0, 0, 0};
+        for (int y = 0; y < splits; ++y) {
+            const float *p = src + (int64_t)y * (BM * (HDP + 2));
+            if (pl.n_t * (int64_t)y / splits == pl.n_t * (int64_t)(y + 1) / splits) continue;     // no keys
+            const float f = __builtin_amdgcn_exp2f(p[col] - ref);
+            l = __builtin_fmaf(p[BM + col], f, l);
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(p + 2 * BM + (int64_t)col * HDP + e);
+#pragma unroll
+            for (int z = 0; z < 4; ++z) acc[z] = __builtin_fmaf(v[z], f, acc[z]);
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int64_t row = pl.s.row0 + i;
+        store4((A *)a.out + row * a.out_stride + (int64_t)hq * a.hd + e, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+        if (a.lse && e == 0) a.lse[row * a.H + hq] = l == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * PK_LN2;
+    }
+}
+
+template <typename T, typename A, typename C, int HDP, int MQ, int QP, int KP, bool PAGED>
+int launch(pk_engine *e, const pk_attn_args &a, int cut, int max_kv) {
+    constexpr int BM = 32 * MQ * TILE_WAVES, KT = tile_keys(HDP, KP);
+    const int64_t G = a.H / a.KVH, slots = (int64_t)a.n_tokens * G / BM + a.n_req, wgs = slots * a.KVH;
+    PK_CHECK(wgs <= INT32_MAX, PK_ERR_UNSUPPORTED, "attention: %lld tiles of rows", (long long)wgs);
+    // two workgroups for every CU, from keys enough for eight tiles each (and
+    // parts for no more than four times as many tile numbers)
+    int splits = 1;
+    const int64_t busy = std::max<int64_t>(((int64_t)a.n_tokens * G + BM - 1) / BM, 1) * a.KVH, want = 2 * e->n_cu;
+    if (PAGED && busy < want) splits = (int)std::max<int64_t>(1, std::min<int64_t>({want / busy, max_kv / (8 * KT), 4 * want / wgs}));
+    float *part = nullptr;
+    if (splits > 1) {
+        PK_TRY(pk_attn_workspace(e, wgs * splits * BM * (HDP + 2), 1));
+        part = e->att_ws;
+    }
+    k_attn_tile<T, A, C, HDP, MQ, QP, KP, PAGED>
+        <<<dim3((unsigned)wgs, (unsigned)splits), TILE_THREADS, 0, e->stream>>>(a, cut, splits, part);
+    PK_HIP(hipGetLastError());
+    if (splits > 1) {
+        k_attn_join<A, BM, HDP, KT><<<dim3((unsigned)wgs, BM / 32), TILE_THREADS, 0, e->stream>>>(a, cut, splits, part);
+        PK_HIP(hipGetLastError());
+    }
+    return PK_OK;
+}
+
+template <typename T, typename A, typename C, int QP, int KP, bool PAGED>
+int by_shape(pk_engine *e, const pk_attn_args &a, int cut, int max_kv) {
+    if (a.hd <= 64) return launch<T, A, C, 64, QP == 1 ? 2 : 1, QP, KP, PAGED>(e, a, cut, max_kv);
+    return launch<T, A, C, 128, 1, QP, KP, PAGED>(e, a, cut, max_kv);
+}
+
+}  // namespace
+
+int pk_launch_attn_tile(pk_engine *e, const pk_attn_args &a, int cut, int max_kv) {
+    if (a.kv_len) {
+        if (a.type == PK_T_F16) return by_shape<pk_f16, pk_f16, pk_f16, 1, 1, true>(e, a, cut, max_kv);
+        if (a.type == PK_T_BF16) return by_shape<pk_bf16, pk_bf16, pk_bf16, 1, 1, true>(e, a, cut, max_kv);
+        if (a.cache_type == PK_T_BF16) return by_shape<pk_bf16, float, pk_bf16, 3, 1, true>(e, a, cut, max_kv);
+        if (a.cache_type == PK_T_F16) return by_shape<pk_bf16, float, pk_f16, 3, 2, true>(e, a, cut, max_kv);
+        return by_shape<pk_bf16, float, float, 3, 3, true>(e, a, cut, max_kv);
+    }
+    if (a.type == PK_T_F16) return by_shape<pk_f16, pk_f16, pk_f16, 1, 1, false>(e, a, cut, max_kv);
+    if (a.type == PK_T_BF16) return by_shape<pk_bf16, pk_bf16, pk_bf16, 1, 1, false>(e, a, cut, max_kv);
+    return by_shape<pk_bf16, float, float, 3, 3, false>(e, a, cut, max_kv);
+}
