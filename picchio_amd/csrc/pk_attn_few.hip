@@ -245,12 +245,15 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_attn_few(pk_attn_args a, flo
             const bool masked = (ok_now & all) != all || base + KT - 1 > p_first || (a.window > 0 && base <= p_last - a.window);
             uint64_t odd = 0;                                   // keys with values that are not finite, seen by some rows only
             if (masked) {
+                // (the empty asm keeps this a branch: as selects it would be work of every tile)
+                uint64_t mine = ok_now >> (4 * g);
+                asm volatile("" : "+v"(mine));
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int jj = b * 16 + 4 * g + i, j = base + jj;
-                        const bool there = ok_now >> jj & 1;
+                        const bool there = mine >> (b * 16 + i) & 1;
 #pragma unroll
                         for (int n = 0; n < NQ; ++n) {
                             const bool see = there && j <= pos[n] && (a.window <= 0 || j > pos[n] - a.window);

@@ -292,18 +292,32 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, i
 #pragma unroll
                         for (int m = 0; m < MQ; ++m) s[m][b] = mfma(kf, q[m][qp][x], s[m][b]);
                 }
-        const bool masked = ok_now != all || base + KT - 1 > w_lo || (a.window > 0 && base <= w_hi - a.window);
-        if (masked) {
+        // (the empty asm keeps these as branches: as selects they would be work of every tile)
+        if (base + KT - 1 > w_lo || (a.window > 0 && base <= w_hi - a.window)) {
+#pragma unroll
+            for (int m = 0; m < MQ; ++m) {
+                int upto = pos[m] - base - 4 * h;
+                asm volatile("" : "+v"(upto));
+                const int from = a.window > 0 ? upto - a.window : -2147483647 - 1;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int kk = b * 32 + 8 * (i >> 2) + (i & 3);
+                        if (kk > upto || kk <= from) s[m][b][i] = -INFINITY;
+                    }
+            }
+        }
+        if (ok_now != all) {
+            uint64_t mine = ok_now >> (4 * h);
+            asm volatile("" : "+v"(mine));
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int kk = b * 32 + 8 * (i >> 2) + 4 * h + (i & 3), j = base + kk;
-                    const bool there = ok_now >> kk & 1;
+                for (int i = 0; i < 16; ++i)
 #pragma unroll
                     for (int m = 0; m < MQ; ++m)
-                        if (!(there && j <= pos[m] && (a.window <= 0 || j > pos[m] - a.window))) s[m][b][i] = -INFINITY;
-                }
+                        if (!(mine >> (b * 32 + 8 * (i >> 2) + (i & 3)) & 1)) s[m][b][i] = -INFINITY;
         }
         // ── probabilities ──
         t8 p[MQ][QP][US];
