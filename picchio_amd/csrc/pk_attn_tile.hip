@@ -25,7 +25,6 @@
 
 namespace {
 
-constexpr int TILE_THREADS = 256, TILE_WAVES = 4;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -39,11 +38,6 @@ struct regs {
 __device__ __forceinline__ f32x16 mfma(pk_f16x8 a, pk_f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma(pk_bf16x8 a, pk_bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-
-template <typename T>
-__device__ __forceinline__ bool not_finite(T v) {
-    return !(__builtin_fabsf((float)v) <= 3.4028234e38f);
 }
 
 // A value's planes: itself in T, or N bf16 that add up to it.
@@ -87,7 +81,7 @@ __device__ __forceinline__ place find(const pk_attn_args &a, int64_t b, int cut,
     }
     __syncthreads();
     place p;
-    p.r = *found;
+    p.r = __builtin_amdgcn_readfirstlane(*found);
     if (p.r < 0) return p;
     p.s = pk_request(a, p.r);
     p.n_idx = min(p.s.rows, a.max_q) * G;
@@ -115,30 +109,105 @@ __device__ __forceinline__ void store4(A *dst, float x, float y, float z, float 
 }
 
 constexpr int tile_keys(int hdp, int kp) { return hdp <= 64 || kp == 1 ? 64 : 32; }
+constexpr int TILE_WAVES = 4, TILE_THREADS = 64 * TILE_WAVES;
 
-template <typename T, typename A, typename C, int HDP, int MQ, int QP, int KP, bool PAGED>
+// 16 bytes per lane from base + off straight to LDS (lane i's at lds + 16 i). In
+// assembly: the compiler does not pair these loads with the kernel's LDS reads
+// (it would wait for every outstanding one before each read); the kernel's own wait
+// and barrier order them. M0 carries the LDS address.
+typedef __attribute__((address_space(3))) void lds_void;
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma16(const void *base, uint32_t off, void *lds) {
+    const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void *)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m), "v"(off), "s"(base) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// Whether one of eight 16-bit values is an infinity or NaN (exponent all ones).
+template <typename T>
+__device__ __forceinline__ uint32_t odd8(const uint4 &v) {
+    constexpr uint32_t E = __is_same(T, pk_f16) ? 0x7c007c00u : 0x7f807f80u, ONE = __is_same(T, pk_f16) ? 0x04000400u : 0x00800080u;
+    return (((v.x & E) + ONE) | ((v.y & E) + ONE) | ((v.z & E) + ONE) | ((v.w & E) + ONE)) & 0x80008000u;
+}
+
+// Element offset of position j's row of keys or values.
+template <bool PAGED>
+__device__ __forceinline__ int64_t row_at(const pk_attn_args &a, const place &pl, int64_t stride, int kvh, int j, bool &there) {
+    if constexpr (PAGED) {
+        const int pg = a.table[(int64_t)pl.r * a.max_blocks + (j >> a.page_shift)];
+        there = pg >= 0 && pg < a.n_pages;
+        return ((((int64_t)(there ? pg : 0) * a.KVH + kvh) << a.page_shift) + (j & ((1 << a.page_shift) - 1))) * a.hd;
+    }
+    there = true;
+    return (pl.s.row0 + (int64_t)j) * stride + kvh * a.hd;
+}
+
+// One column over the keys from..to, a wave at a time, position by position: for
+// workgroups that met values of V that are not finite where some row does not
+// see them (0 x infinity in a product), which then do all their columns so.
+template <typename A, typename C, int BM, bool PAGED>
+__device__ __attribute__((noinline)) void slow_column(pk_attn_args a, place pl, int kvh, int idx, int from, int to, bool whole,
+                                                      float *part_m, float *part_o) {
+    const int lane = threadIdx.x & 63, G = a.H / a.KVH, hd = a.hd, i = idx / G, h = kvh * G + (idx - i * G);
+    const int p = pl.s.kv - pl.s.rows + i;
+    const int64_t row = pl.s.row0 + i;
+    const A *q = (const A *)a.q + row * a.q_stride + (int64_t)h * hd;
+    const float sk = whole && a.sinks ? a.sinks[h] * PK_LOG2E : -INFINITY;
+    float m = sk, l = whole && a.sinks && sk > -INFINITY ? 1.0f : 0.0f, o0 = 0.0f, o1 = 0.0f;
+    const int lo = a.window > 0 ? max(from, p - a.window + 1) : from, hi = min(to, p + 1);
+    for (int j = lo; j < hi; ++j) {
+        bool there;
+        const C *k = (const C *)a.k + row_at<PAGED>(a, pl, a.k_stride, kvh, j, there);
+        const C *v = (const C *)a.v + row_at<PAGED>(a, pl, a.v_stride, kvh, j, there);
+        if (!there) continue;
+        float s = 0.0f;
+        if (lane < hd) s = (float)q[lane] * (float)k[lane];
+        if (lane + 64 < hd) s = __builtin_fmaf((float)q[lane + 64], (float)k[lane + 64], s);
+        s = pk_wave_sum_f(s) * a.scale2;
+        const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
+        const float f = __builtin_amdgcn_exp2f(m - ref), e = __builtin_amdgcn_exp2f(s - ref);
+        m = mn;
+        l = __builtin_fmaf(l, f, e);
+        o0 = __builtin_fmaf(e, lane < hd ? (float)v[lane] : 0.0f, o0 * f);
+        o1 = __builtin_fmaf(e, lane + 64 < hd ? (float)v[lane + 64] : 0.0f, o1 * f);
+    }
+    if (whole) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        A *dst = (A *)a.out + row * a.out_stride + (int64_t)h * hd;
+        if (lane < hd) dst[lane] = (A)(o0 * inv);
+        if (lane + 64 < hd) dst[lane + 64] = (A)(o1 * inv);
+        if (a.lse && lane == 0) a.lse[row * a.H + h] = l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) + __builtin_amdgcn_logf(l)) * PK_LN2;
+    } else {
+        if (lane == 0) part_m[0] = m, part_m[BM] = l;
+        if (lane < hd) part_o[lane] = o0;
+        if (lane + 64 < hd) part_o[lane + 64] = o1;
+    }
+}
+
+template <typename T, typename A, typename C, int HDP, int MQ, int QP, int KP, bool PAGED, bool FULL>
 __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, int cut, int splits, float *part) {
     constexpr int KT = tile_keys(HDP, KP), BM = 32 * MQ * TILE_WAVES;
     constexpr int NB = KT / 32, QS = HDP / 16, HT = HDP / 32, US = KT / 16;
-    constexpr int CPR = HDP / 8, RPP = TILE_THREADS / CPR, NP = KT / RPP, ROWB = HDP * 2;
+    // a tile's 16-byte pieces: CPR to a row, KPW rows to a wave, RPP to a pass of the workgroup
+    constexpr int CPR = HDP / 8, KPW = 64 / CPR, RPP = TILE_THREADS / CPR, NP = KT / RPP, ROWB = HDP * 2;
     constexpr bool PLANES = QP > 1;
+    constexpr int BUFS = PLANES ? 1 : 2;                        // direct loads need the next tile's place too
+    constexpr uint64_t ALL = KT == 64 ? ~0ull : (1ull << KT) - 1;
     typedef typename regs<T, 8>::type t8;
     typedef typename regs<C, 8>::type c8;
     typedef typename regs<A, 8>::type a8;
 
-    __shared__ __attribute__((aligned(16))) uint8_t sK[KP][KT * ROWB], sV[KP][KT * ROWB];
-    __shared__ unsigned long long odd_keys[2];
+    __shared__ __attribute__((aligned(16))) uint8_t sK[BUFS][KP][KT * ROWB], sV[BUFS][KP][KT * ROWB];
     __shared__ int found;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, c32 = lane & 31;
-    const int kvh = blockIdx.x % a.KVH, G = a.H / a.KVH, hd = a.hd;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, c32 = lane & 31;
+    const int kvh = blockIdx.x % a.KVH, G = a.H / a.KVH, hd = FULL ? HDP : a.hd;
     const int64_t slot = blockIdx.x / a.KVH;
     const place pl = find<BM, KT>(a, slot, cut, &found);
     if (pl.r < 0) return;
     const int t_first = (int)((int64_t)pl.n_t * blockIdx.y / splits), t_end = (int)((int64_t)pl.n_t * (blockIdx.y + 1) / splits);
     const int before = pl.s.kv - pl.s.rows, end = pl.p_hi + 1;
-    const int32_t *tab = PAGED ? a.table + (int64_t)pl.r * a.max_blocks : nullptr;
-    const int ps = PAGED ? 1 << a.page_shift : 0;
 
     // ── queries ──
     t8 q[MQ][QP][QS];
@@ -146,6 +215,10 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, i
     const int w0 = pl.idx0 + wave * 32 * MQ;                    // the wave's first column
     const bool active = w0 < pl.n_idx;
     const int w_lo = before + w0 / G, w_hi = before + (min(w0 + 32 * MQ, pl.n_idx) - 1) / G;
+    // keys at or below p_old (w_old) lie outside the window of some row of the workgroup
+    // (the wave), below w_none of every row of the wave
+    const int p_old = a.window > 0 ? pl.p_hi - a.window : -1;
+    const int w_old = a.window > 0 ? w_hi - a.window : -1, w_none = a.window > 0 ? w_lo - a.window : -1;
 #pragma unroll
     for (int m = 0; m < MQ; ++m) {
         const int idx = w0 + m * 32 + c32, i = idx / G;
@@ -163,6 +236,8 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, i
             for (int n = 0; n < QP; ++n) q[m][n][s] = p[n];
         }
     }
+    float scale2 = a.scale2;
+    asm volatile("" : "+v"(scale2));                            // (a register: or it is loaded anew for every tile)
 
     f32x16 o[MQ][HT];
     float mx[MQ], ls[MQ];
@@ -176,100 +251,124 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, i
             for (int i = 0; i < 16; ++i) o[m][x][i] = 0.0f;
     }
 
-    // ── staging: this thread's pieces of a tile's keys and values ──
-    const int my_key = tid / CPR, my_c = tid % CPR;
-    c8 rk[NP], rv[NP];
+    // ── staging ──
+    // A wave's share of a pass is KPW neighbouring rows, which lie on one page: their
+    // address is a scalar, a lane's offset from it the same for every tile. Piece c
+    // of row r is kept at place c ^ f(r): f(r) = r % 8 for K (32 lanes read a piece of 32
+    // rows), 2 (r % 4) for V (16 lanes read two pieces of four rows).
+    const int my_row = lane / CPR, my_c = lane % CPR, my_key = wave * KPW + my_row;
+    const int ck = PLANES ? my_c : my_c ^ (my_key & 7), cv = PLANES ? my_c : my_c ^ ((my_key & 3) << 1);
+    const int64_t rowk = PAGED ? hd : a.k_stride, rowv = PAGED ? hd : a.v_stride;
+    const uint32_t offk = (uint32_t)(my_row * rowk + (ck * 8 < hd ? ck * 8 : 0)) * (uint32_t)sizeof(C);
+    const uint32_t offv = (uint32_t)(my_row * rowv + (cv * 8 < hd ? cv * 8 : 0)) * (uint32_t)sizeof(C);
+    // Page of position base + lane of tile t, and the bits of the positions that there are.
     const auto look = [&](int t, uint64_t &ok) {
-        const int j = pl.first + t * KT + (lane & (KT - 1));
-        int pg = 0;
-        bool good = j < end;
+        const int base = pl.first + t * KT;
         if constexpr (PAGED) {
-            pg = tab[min(j, max(end - 1, 0)) >> a.page_shift];
-            good = good && pg >= 0 && pg < a.n_pages;
-            pg = good ? pg : 0;
+            const int j = base + (lane & (KT - 1));
+            const int pg = a.table[(int64_t)pl.r * a.max_blocks + (min(j, max(end - 1, 0)) >> a.page_shift)];
+            const bool good = j < end && pg >= 0 && pg < a.n_pages;
+            ok = __ballot(good) & ALL;
+            return good ? pg : 0;
+        } else {
+            ok = end - base >= KT ? ALL : (1ull << max(end - base, 0)) - 1;
+            return 0;
         }
-        ok = __ballot(good);
-        return pg;
     };
-    const auto load = [&](int t, int pgs) {
-        const int base = pl.first + t * KT, e = my_c * 8 < hd ? my_c * 8 : 0;
+    c8 rk[PLANES ? NP : 1], rv[PLANES ? NP : 1];
+    const auto load = [&](int t, int pgs, uint64_t ok) {
+        const int base = pl.first + t * KT, buf = t & (BUFS - 1);
+        uint32_t ok_ = offk, ov_ = offv;
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
-            const int kk = n * RPP + my_key, j = base + kk;
+            const int k0 = n * RPP + wave * KPW, j0 = base + k0;
             int64_t ak, av;
             if constexpr (PAGED) {
-                const int pg = __shfl(pgs, kk);
-                ak = av = ((((int64_t)pg * a.KVH + kvh) << a.page_shift) + (j & (ps - 1))) * hd + e;
+                const int pg = __builtin_amdgcn_readlane(pgs, k0);
+                ak = av = ((((int64_t)pg * a.KVH + kvh) << a.page_shift) + (j0 & ((1 << a.page_shift) - 1))) * hd;
             } else {
-                const int64_t row = pl.s.row0 + min(j, end - 1);
-                ak = row * a.k_stride + kvh * hd + e;
-                av = row * a.v_stride + kvh * hd + e;
+                ak = (pl.s.row0 + (int64_t)min(j0, end - 1)) * rowk + kvh * hd;
+                av = (pl.s.row0 + (int64_t)min(j0, end - 1)) * rowv + kvh * hd;
+                if (ok != ALL) {                                // no row behind the prompt's last one
+                    int back = my_row - min(my_row, max(end - 1 - j0, 0));
+                    asm volatile("" : "+v"(back));
+                    ok_ = offk - (uint32_t)(back * rowk) * (uint32_t)sizeof(C);
+                    ov_ = offv - (uint32_t)(back * rowv) * (uint32_t)sizeof(C);
+                }
             }
-            rk[n] = *reinterpret_cast<const c8 *>((const C *)a.k + ak);
-            rv[n] = *reinterpret_cast<const c8 *>((const C *)a.v + av);
+            const char *pk = (const char *)((const C *)a.k + ak), *pv = (const char *)((const C *)a.v + av);
+            if constexpr (PLANES) {
+                rk[n] = *reinterpret_cast<const c8 *>(pk + ok_);
+                rv[n] = *reinterpret_cast<const c8 *>(pv + ov_);
+            } else {
+                dma16(pk, ok_, &sK[buf][0][k0 * ROWB]);
+                dma16(pv, ov_, &sV[buf][0][k0 * ROWB]);
+            }
         }
     };
     uint64_t ok = 0, ok_next = 0;
     int pgs_next = 0;
     if (t_first < t_end) {
         const int pgs = look(t_first, ok);
-        load(t_first, pgs);
+        load(t_first, pgs, ok);
         if (t_first + 1 < t_end) pgs_next = look(t_first + 1, ok_next);
     }
-    if (tid < 2) odd_keys[tid] = 0;
+    uint32_t odd = 0;                                           // this thread met a value that calls for slow_column
 
     for (int t = t_first; t < t_end; ++t) {
-        const int base = pl.first + t * KT;
-        const uint64_t all = KT == 64 ? ~0ull : (1ull << KT) - 1, ok_now = ok & all;
+        const int base = pl.first + t * KT, buf = t & (BUFS - 1);
+        const uint64_t ok_now = ok;
         // a tile that some row of the workgroup does not see whole
-        const bool edge = ok_now != all || base + KT - 1 > pl.p_lo || (a.window > 0 && base <= pl.p_hi - a.window);
-        __syncthreads();                                        // the previous tile has been read
+        const bool edge = ok_now != ALL || base + KT - 1 > pl.p_lo || base <= p_old;
+        if constexpr (PLANES) {
+            __syncthreads();                                    // the previous tile has been read
 #pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            const int kk = n * RPP + my_key;
-            if (!(ok_now >> kk & 1) || my_c * 8 >= hd) rk[n] = c8{}, rv[n] = c8{};
-            if (edge || PLANES) {
-                // values that are not finite and that some rows do not see (with
-                // planes: any): left out here, added one by one below
-                bool bad = false;
+            for (int n = 0; n < NP; ++n) {
+                const int kk = n * RPP + my_key;
+                if (ok_now != ALL) {
+                    uint64_t mine = ok_now;
+                    asm volatile("" : "+v"(mine));
+                    if (!(mine >> kk & 1)) rk[n] = c8{}, rv[n] = c8{};
+                }
+                float sum = 0.0f;                               // (finite values: 0)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) bad |= not_finite(rv[n][i]);
-                if (bad) {
-                    const int j = base + kk;
-                    if (PLANES || j > pl.p_lo || (a.window > 0 && j <= pl.p_hi - a.window)) atomicOr(&odd_keys[t & 1], 1ull << kk);
+                for (int i = 0; i < 8; ++i) sum = __builtin_fmaf((float)rv[n][i], 0.0f, sum);
+                if (my_c * 8 < hd) odd |= sum != 0.0f;
+                t8 pk[KP], pv[KP];
+                planes<T, KP>(rk[n], pk);
+                planes<T, KP>(rv[n], pv);
+#pragma unroll
+                for (int x = 0; x < KP; ++x) {
+                    *reinterpret_cast<t8 *>(&sK[0][x][kk * ROWB + ((my_c ^ (kk & 7)) << 4)]) = pk[x];
+                    *reinterpret_cast<t8 *>(&sV[0][x][kk * ROWB + ((my_c ^ ((kk & 3) << 1)) << 4)]) = pv[x];
                 }
             }
-            t8 pk[KP], pv[KP];
-            planes<T, KP>(rk[n], pk);
-            planes<T, KP>(rv[n], pv);
-#pragma unroll
-            for (int x = 0; x < KP; ++x) {
-                *reinterpret_cast<t8 *>(&sK[x][kk * ROWB + ((my_c ^ (kk & 7)) << 4)]) = pk[x];
-                *reinterpret_cast<t8 *>(&sV[x][kk * ROWB + ((my_c ^ ((kk & 3) << 1)) << 4)]) = pv[x];
-            }
+            __syncthreads();
+        } else {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0x0f70);                 // vmcnt(0): the wave's part of this tile is in LDS
+            __syncthreads();
         }
-        __syncthreads();
-        uint64_t odd = 0;
-        if (edge || PLANES) {
-            odd = odd_keys[t & 1];
-            if (odd) {                                          // (rare) their rows of V: zero
-                __syncthreads();
-                for (uint64_t left = odd; left; left &= left - 1) {
-                    const int kk = __ffsll((unsigned long long)left) - 1;
-                    for (int x = tid; x < KP * CPR; x += TILE_THREADS)
-                        *reinterpret_cast<t8 *>(&sV[x / CPR][kk * ROWB + ((x % CPR) << 4)]) = t8{};
-                }
-                __syncthreads();
-            }
-        }
-        if (tid == 0) odd_keys[(t + 1) & 1] = 0;
         if (t + 1 < t_end) {
-            load(t + 1, pgs_next);
+            load(t + 1, pgs_next, ok_next);
             ok = ok_next;
             if (t + 2 < t_end) pgs_next = look(t + 2, ok_next);
         }
+        if (!PLANES && edge) {
+            // rows that are not there: zero (0 x NaN); values that are not finite, on rows that not all see
+            uint64_t mine = ok_now >> my_key;
+            asm volatile("" : "+v"(mine));
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                uint4 *pv = reinterpret_cast<uint4 *>(&sV[buf][0][(n * RPP + wave * KPW) * ROWB + lane * 16]);
+                const int j = base + n * RPP + my_key;
+                if (!(mine >> (n * RPP) & 1)) *pv = uint4{0, 0, 0, 0};
+                else if (j > pl.p_lo || j <= p_old) odd |= odd8<T>(*pv);
+            }
+            if (ok_now != ALL) __syncthreads();
+        }
         // a tile that the wave's rows do not see at all
-        if (!active || base > w_hi || (a.window > 0 && base + KT - 1 <= w_lo - a.window)) continue;
+        if (!active || base > w_hi || base + KT - 1 <= w_none) continue;
 
         // ── S^T = K Q^T ──
         f32x16 s[MQ][NB];
@@ -280,20 +379,22 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, i
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[m][b][i] = 0.0f;
 #pragma unroll
-        for (int x = 0; x < QS; ++x)
+        for (int x = 0; x < QS; ++x) {
+            if (!FULL && 16 * x >= hd) break;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int kp = 0; kp < KP; ++kp) {
                     const int kk = b * 32 + c32;
-                    const t8 kf = *reinterpret_cast<const t8 *>(&sK[kp][kk * ROWB + (((2 * x + h) ^ (kk & 7)) << 4)]);
+                    const t8 kf = *reinterpret_cast<const t8 *>(&sK[buf][kp][kk * ROWB + (((2 * x + h) ^ (kk & 7)) << 4)]);
 #pragma unroll
                     for (int qp = 0; qp < QP && qp + kp < 3; ++qp)
 #pragma unroll
                         for (int m = 0; m < MQ; ++m) s[m][b] = mfma(kf, q[m][qp][x], s[m][b]);
                 }
+        }
         // (the empty asm keeps these as branches: as selects they would be work of every tile)
-        if (base + KT - 1 > w_lo || (a.window > 0 && base <= w_hi - a.window)) {
+        if (base + KT - 1 > w_lo || base <= w_old) {
 #pragma unroll
             for (int m = 0; m < MQ; ++m) {
                 int upto = pos[m] - base - 4 * h;
@@ -308,7 +409,7 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, i
                     }
             }
         }
-        if (ok_now != all) {
+        if (PAGED && ok_now != ALL) {
             uint64_t mine = ok_now >> (4 * h);
             asm volatile("" : "+v"(mine));
 #pragma unroll
@@ -330,7 +431,7 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, i
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[m][b][i]);
             {
                 const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-                top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * a.scale2;
+                top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * scale2;
             }
             // the reference only moves when a score is 2^8 above it: what
             // lies between makes sums and probabilities no less exact
@@ -347,7 +448,7 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, i
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[m][b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][b][i], a.scale2, -ref));
+                    s[m][b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][b][i], scale2, -ref));
                     sum += s[m][b][i];
                 }
             ls[m] += sum;
@@ -363,59 +464,39 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, i
             }
         }
         // ── O^T += V^T P^T: the keys of step u in the order of the scores' registers ──
-        {
-            const int kr = 4 * h + ((lane & 15) >> 2), c0 = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), sub = (lane & 1) << 3;
-            const int sw = (kr & 3) << 1;
+        const int kr = 4 * h + ((lane & 15) >> 2), c0 = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), sub = (lane & 1) << 3;
+        const int sw = (kr & 3) << 1;
 #pragma unroll
-            for (int u = 0; u < US; ++u)
+        for (int u = 0; u < US; ++u)
 #pragma unroll
-                for (int x = 0; x < HT; ++x)
+            for (int x = 0; x < HT; ++x) {
+                if (!FULL && 32 * x >= hd) break;
 #pragma unroll
-                    for (int kp = 0; kp < KP; ++kp) {
-                        const int at = (16 * u + kr) * ROWB + (((4 * x + c0) ^ sw) << 4) + sub;
-                        typedef __attribute__((address_space(3))) s16x4 lds4;
-                        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)&sV[kp][at]);
-                        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)&sV[kp][at + 8 * ROWB]);
-                        typename regs<short, 8>::type vv;
+                for (int kp = 0; kp < KP; ++kp) {
+                    const int at = (16 * u + kr) * ROWB + (((4 * x + c0) ^ sw) << 4) + sub;
+                    typedef __attribute__((address_space(3))) s16x4 lds4;
+                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)&sV[buf][kp][at]);
+                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)&sV[buf][kp][at + 8 * ROWB]);
+                    typename regs<short, 8>::type vv;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) vv[i] = v0[i], vv[4 + i] = v1[i];
-                        const t8 vf = __builtin_bit_cast(t8, vv);
+                    for (int i = 0; i < 4; ++i) vv[i] = v0[i], vv[4 + i] = v1[i];
+                    const t8 vf = __builtin_bit_cast(t8, vv);
 #pragma unroll
-                        for (int qp = 0; qp < QP && qp + kp < 3; ++qp)
+                    for (int qp = 0; qp < QP && qp + kp < 3; ++qp)
 #pragma unroll
-                            for (int m = 0; m < MQ; ++m) o[m][x] = mfma(vf, p[m][qp][u], o[m][x]);
-                    }
-        }
-        // ── values that are not finite, on the rows that see them ──
-        while (odd) {
-            const int kk = __ffsll((unsigned long long)odd) - 1, j = base + kk;
-            odd &= odd - 1;
-            int64_t at;
-            if constexpr (PAGED) at = ((((int64_t)tab[j >> a.page_shift] * a.KVH + kvh) << a.page_shift) + (j & (ps - 1))) * hd;
-            else at = (int64_t)(pl.s.row0 + j) * a.v_stride + kvh * hd;
-            const C *src = (const C *)a.v + at;
-#pragma unroll
-            for (int m = 0; m < MQ; ++m) {
-                float pr = 0.0f;
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (b == kk >> 5 && i == 4 * ((kk & 31) >> 3) + (kk & 3)) pr = s[m][b][i];
-                pr = __shfl(pr, c32 + 32 * ((kk >> 2) & 1));
-                if (j <= pos[m] && (a.window <= 0 || j > pos[m] - a.window))
-#pragma unroll
-                    for (int x = 0; x < HT; ++x)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int e = 32 * x + 8 * (i >> 2) + 4 * h + (i & 3);
-                            if (e < hd) o[m][x][i] = __builtin_fmaf(pr, (float)src[e], o[m][x][i]);
-                        }
+                        for (int m = 0; m < MQ; ++m) o[m][x] = mfma(vf, p[m][qp][u], o[m][x]);
+                }
             }
-        }
     }
 
     // ── out ──
+    float *dst_part = part + ((slot * a.KVH + kvh) * splits + blockIdx.y) * (BM * (HDP + 2));
+    if (__syncthreads_or((int)odd)) {
+        for (int col = wave; col < BM && pl.idx0 + col < pl.n_idx; col += TILE_WAVES)
+            slow_column<A, C, BM, PAGED>(a, pl, kvh, pl.idx0 + col, pl.first + t_first * KT, pl.first + t_end * KT, splits == 1,
+                                         dst_part + col, dst_part + 2 * BM + (int64_t)col * HDP);
+        return;
+    }
 #pragma unroll
     for (int m = 0; m < MQ; ++m) {
         const int col = wave * 32 * MQ + m * 32 + c32, idx = pl.idx0 + col;
@@ -445,8 +526,7 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, i
                 }
             if (a.lse && h == 0) a.lse[row * a.H + hq] = l == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * PK_LN2;
         } else {
-            float *dst = part + ((slot * a.KVH + kvh) * splits + blockIdx.y) * (BM * (HDP + 2));
-            if (h == 0) dst[col] = mx[m], dst[BM + col] = l;
+            if (h == 0) dst_part[col] = mx[m], dst_part[BM + col] = l;
             if (t_first < t_end)
 #pragma unroll
                 for (int x = 0; x < HT; ++x)
@@ -454,7 +534,7 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, i
                     for (int y = 0; y < 4; ++y) {
                         const int e = 32 * x + 8 * y + 4 * h;
                         if (e < hd)
-                            store4(dst + 2 * BM + (int64_t)col * HDP + e, o[m][x][4 * y], o[m][x][4 * y + 1], o[m][x][4 * y + 2],
+                            store4(dst_part + 2 * BM + (int64_t)col * HDP + e, o[m][x][4 * y], o[m][x][4 * y + 1], o[m][x][4 * y + 2],
                                    o[m][x][4 * y + 3]);
                     }
         }
@@ -462,8 +542,9 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_tile(pk_attn_args a, i
 }
 
 // The parts of split keys, added up in order: four elements of a column per thread.
+constexpr int JOIN_THREADS = 256;
 template <typename A, int BM, int HDP, int KT>
-__global__ __launch_bounds__(TILE_THREADS) void k_attn_join(pk_attn_args a, int cut, int splits, const float *__restrict__ part) {
+__global__ __launch_bounds__(JOIN_THREADS) void k_attn_join(pk_attn_args a, int cut, int splits, const float *__restrict__ part) {
     __shared__ int found;
     const int kvh = blockIdx.x % a.KVH, G = a.H / a.KVH, quads = a.hd >> 2;
     const int64_t slot = blockIdx.x / a.KVH;
@@ -471,7 +552,7 @@ __global__ __launch_bounds__(TILE_THREADS) void k_attn_join(pk_attn_args a, int 
     if (pl.r < 0) return;
     const float *src = part + (slot * a.KVH + kvh) * splits * (BM * (HDP + 2));
     const int cols = min(BM, pl.n_idx - pl.idx0);
-    for (int x = blockIdx.y * TILE_THREADS + threadIdx.x; x < cols * quads; x += gridDim.y * TILE_THREADS) {
+    for (int x = blockIdx.y * JOIN_THREADS + threadIdx.x; x < cols * quads; x += gridDim.y * JOIN_THREADS) {
         const int col = x / quads, e = (x - col * quads) * 4, idx = pl.idx0 + col, i = idx / G, hq = kvh * G + (idx - i * G);
         const float sk = a.sinks ? a.sinks[hq] * PK_LOG2E : -INFINITY;
         float top = sk;
@@ -495,8 +576,8 @@ __global__ __launch_bounds__(TILE_THREADS) void k_attn_join(pk_attn_args a, int 
     }
 }
 
-template <typename T, typename A, typename C, int HDP, int MQ, int QP, int KP, bool PAGED>
-int launch(pk_engine *e, const pk_attn_args &a, int cut, int max_kv) {
+template <typename T, typename A, typename C, int HDP, int MQ, int QP, int KP, bool PAGED, bool FULL>
+int launch_as(pk_engine *e, const pk_attn_args &a, int cut, int max_kv) {
     constexpr int BM = 32 * MQ * TILE_WAVES, KT = tile_keys(HDP, KP);
     const int64_t G = a.H / a.KVH, slots = (int64_t)a.n_tokens * G / BM + a.n_req, wgs = slots * a.KVH;
     PK_CHECK(wgs <= INT32_MAX, PK_ERR_UNSUPPORTED, "attention: %lld tiles of rows", (long long)wgs);
@@ -510,14 +591,20 @@ int launch(pk_engine *e, const pk_attn_args &a, int cut, int max_kv) {
         PK_TRY(pk_attn_workspace(e, wgs * splits * BM * (HDP + 2), 1));
         part = e->att_ws;
     }
-    k_attn_tile<T, A, C, HDP, MQ, QP, KP, PAGED>
+    k_attn_tile<T, A, C, HDP, MQ, QP, KP, PAGED, FULL>
         <<<dim3((unsigned)wgs, (unsigned)splits), TILE_THREADS, 0, e->stream>>>(a, cut, splits, part);
     PK_HIP(hipGetLastError());
     if (splits > 1) {
-        k_attn_join<A, BM, HDP, KT><<<dim3((unsigned)wgs, BM / 32), TILE_THREADS, 0, e->stream>>>(a, cut, splits, part);
+        k_attn_join<A, BM, HDP, KT><<<dim3((unsigned)wgs, BM / 32), JOIN_THREADS, 0, e->stream>>>(a, cut, splits, part);
         PK_HIP(hipGetLastError());
     }
     return PK_OK;
+}
+
+template <typename T, typename A, typename C, int HDP, int MQ, int QP, int KP, bool PAGED>
+int launch(pk_engine *e, const pk_attn_args &a, int cut, int max_kv) {
+    return a.hd == HDP ? launch_as<T, A, C, HDP, MQ, QP, KP, PAGED, true>(e, a, cut, max_kv)
+                       : launch_as<T, A, C, HDP, MQ, QP, KP, PAGED, false>(e, a, cut, max_kv);
 }
 
 template <typename T, typename A, typename C, int QP, int KP, bool PAGED>
