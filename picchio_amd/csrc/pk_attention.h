@@ -52,7 +52,7 @@ int pk_attn_workspace(pk_engine *e, int64_t floats, int64_t counts);
 // Rows of a request times query heads per KV head that one launch of k_attn_few
 // holds; the launchers.
 constexpr int PK_FEW_ROWS = 32;
-int pk_launch_attn_few(pk_engine *e, const pk_attn_args &a, int max_kv);
+int pk_launch_attn_few(pk_engine *e, const pk_attn_args &a);
 // Requests with more than `cut` of these (the rest is k_attn_few's).
 int pk_launch_attn_tile(pk_engine *e, const pk_attn_args &a, int cut, int max_kv);
 

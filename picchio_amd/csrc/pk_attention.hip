@@ -89,13 +89,13 @@ extern "C" int pk_attention_paged(pk_engine *e, const pk_attn_paged *p) {
     // requests with few rows there (a tile of 128 or 256 columns would be
     // mostly empty for them), the others in tiles.
     const int G = a.H / a.KVH;
-    if ((int64_t)a.max_q * G <= PK_FEW_ROWS) return pk_launch_attn_few(e, a, max_kv);
+    if ((int64_t)a.max_q * G <= PK_FEW_ROWS) return pk_launch_attn_few(e, a);
     int cut = 0;
     if (a.n_req > 1 && G <= PK_FEW_ROWS) {
         cut = G <= 16 ? 16 : PK_FEW_ROWS;
         pk_attn_args few = a;
         few.max_q = cut / G, few.few_only = 1;
-        PK_TRY(pk_launch_attn_few(e, few, max_kv));
+        PK_TRY(pk_launch_attn_few(e, few));
     }
     return pk_launch_attn_tile(e, a, cut, max_kv);
 }

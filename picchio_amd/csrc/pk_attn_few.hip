@@ -9,12 +9,14 @@
 // product, and of the keys in the second, is free, so that both operands are
 // loaded straight from the pages, 8 or 16 bytes per lane, with no LDS between.
 //
-// The positions of all requests, in tiles of KT, lie behind each other on one
-// line, of which each workgroup takes an equal share (per KV head), whatever
-// the requests' lengths; its waves take every fourth tile. A request that ends
-// inside one share is written out there; of one that spans several, each
-// workgroup leaves its part, and the one that arrives last joins them in the
-// line's order.
+// The tiles of KT positions of all requests, U of them, are cut into chunks of
+// about U / W: a request of up to a chunk is one item, a longer one several of
+// equal length. A workgroup (per KV head) is one item, whatever the requests'
+// lengths, and its waves take every fourth tile of it. Of a request of several
+// items each leaves its part, and the workgroup that arrives last joins them in
+// order. (Equal shares of one line of tiles instead, across requests, left a
+// workgroup with the parts of several, one after the other: 32 requests with
+// 128-position windows 23 us, as items 12.)
 #include "pk_attention.h"
 
 namespace {
@@ -36,16 +38,50 @@ __device__ __forceinline__ f32x4 mfma(pk_bf16x8 a, pk_bf16x8 b, f32x4 c) {
 }
 __device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
-// Positions per tile: a wave has a tile's keys (also the next one's) and values in
-// registers, 256 of them per lane with two columns' worth of everything else.
-constexpr int few_tile(int row_bytes, int nq) { return row_bytes <= 128 ? 64 / nq : row_bytes <= 256 ? 32 : 16; }
-
-template <typename T>
-__device__ __forceinline__ bool not_finite(T v) {
-    return !(__builtin_fabsf((float)v) <= 3.4028234e38f);
+// A value's planes: itself in T, or N values of T that add up to it (cut to 8 bits each
+// for bf16; for fp16 rounded, the second the rest).
+template <typename T, int N, typename V8>
+__device__ __forceinline__ void planes(const V8 &x, typename regs<T, 8>::type (&p)[N]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (N == 1) {
+            p[0][i] = (T)x[i];
+        } else if constexpr (N == 2) {
+            p[0][i] = (T)(float)x[i];
+            p[1][i] = (T)((float)x[i] - (float)p[0][i]);
+        } else {
+            float v = (float)x[i];
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const uint32_t hi = __float_as_uint(v) & 0xffff0000u;
+                p[n][i] = __builtin_bit_cast(T, (uint16_t)(hi >> 16));
+                v = v - __uint_as_float(hi);
+            }
+        }
+    }
 }
 
-// The tiles of a request, and of those before it, on the line.
+// Positions per tile: a wave has a tile's keys (also the next one's) and values in
+// registers, 256 of them per lane with two columns' worth of everything else.
+// (32 positions where 64 fit: one row over 100,001 positions, fp32 over fp16, 63 us for 52; with
+// three workgroups on a CU 59.)
+constexpr int few_tile(int row_bytes, int nq) { return row_bytes <= 128 ? 64 / nq : row_bytes <= 256 ? 32 : 16; }
+constexpr int FEW_PER_CU = 2;
+
+// Not 0 where one of N values is an infinity or NaN (exponent all ones).
+template <typename T, int N>
+__device__ __forceinline__ uint32_t odd_row(const typename regs<T, N>::type &v) {
+    constexpr uint32_t E = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, pk_f16) ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t ONE = sizeof(T) == 4 ? 0x00800000u : __is_same(T, pk_f16) ? 0x04000400u : 0x00800080u;
+    constexpr uint32_t TOP = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+    const auto w = __builtin_bit_cast(typename regs<uint32_t, N * (int)sizeof(T) / 4>::type, v);
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < N * (int)sizeof(T) / 4; ++i) any |= (w[i] & E) + ONE;
+    return any & TOP;
+}
+
+// A request's tiles.
 struct seg {
     pk_span s;
     int first, tiles;          // first position (a multiple of KT), tiles (0: no rows; at least 1 otherwise)
@@ -60,17 +96,34 @@ __device__ __forceinline__ seg few_seg(const pk_attn_args &a, int r) {
     return g;
 }
 
-// Share of the line: worker w of W takes tiles [w U / W, (w + 1) U / W).
-__device__ __forceinline__ int64_t share(int64_t U, int w, int W) { return U * w / W; }
-// The worker that has tile u.
-__device__ __forceinline__ int owner(int64_t u, int64_t U, int W) {
-    int w = (int)(((u + 1) * W - 1) / U);                       // share(w) <= u < share(w + 1)
-    return w;
+constexpr int FEW_TRIES = 8;
+__device__ __forceinline__ int try_chunk(int64_t share, int k) {
+    return (int)min(share + share * (k < 5 ? k : 2 * k - 4) / 8, (int64_t)INT32_MAX / 2);     // 1, 9/8 .. 12/8, 14/8, 2, 18/8
+}
+
+// Sums over the lanes up to this one.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, true);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v = dpp_add<0x111, 0xf>(v);                                // row_shr 1, 2, 4, 8
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);                                // lane 15 of a row to the next row, 31 to the upper half
+    return dpp_add<0x143, 0xc>(v);
 }
 
 template <typename A, typename C, int HDP, int NQ>
-__global__ __launch_bounds__(FEW_THREADS, 2) void k_attn_few(pk_attn_args a, float *part, uint32_t *count) {
-    constexpr bool F32 = sizeof(A) == 4;                        // fp32 products, the cache widened
+__global__ __launch_bounds__(FEW_THREADS, FEW_PER_CU) void k_attn_few(pk_attn_args a, int W, int max_parts, float *part, uint32_t *count) {
+    constexpr bool F32 = sizeof(C) == 4;                        // fp32 cache: fp32 products
+    // fp32 queries and probabilities over a 16-bit cache: as planes of the cache's type, whose
+    // products are exact. bf16: three, 8 bits each. fp16: two, 11 bits each, of values
+    // scaled to at most 2^14, so that the low plane's last bit is at 2^-38 of that.
+    constexpr int QP = F32 || sizeof(A) == 2 ? 1 : __is_same(C, pk_f16) ? 2 : 3;
+    constexpr float SHIFT = __is_same(C, pk_f16) ? 14.0f : 0.0f;    // probabilities are at most 2^SHIFT
+    typedef typename regs<C, 8>::type c8;
     constexpr int KT = few_tile(HDP * (int)sizeof(C), NQ), NB = KT / 16;
     constexpr int KE = HDP / 4, KV8 = KE / 8;                   // elements of a key per lane, in vectors of 8
     constexpr int VE = HDP / 16;                                // elements of a value per lane
@@ -80,75 +133,103 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_attn_few(pk_attn_args a, flo
 
     __shared__ __attribute__((aligned(16))) float so[FEW_WAVES][COLS][LD];
     __shared__ float sm[FEW_WAVES][COLS], sl[FEW_WAVES][COLS];
-    __shared__ int64_t line[FEW_THREADS / 64 + 1];
-    __shared__ int64_t start_at;
-    __shared__ int start_r, last_in;
+    __shared__ int last_in;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m16 = lane & 15;
-    const int W = gridDim.x, kvh = blockIdx.y, G = a.H / a.KVH, hd = a.hd;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m16 = lane & 15;
+    const int kvh = blockIdx.y, G = a.H / a.KVH, hd = a.hd;
     const int ps = 1 << a.page_shift;
 
-    // ── this workgroup's share of the line ──
-    const int per = (a.n_req + FEW_THREADS - 1) / FEW_THREADS;
-    int64_t mine = 0;
-    for (int i = 0; i < per; ++i)
-        if (tid * per + i < a.n_req) mine += few_seg<KT>(a, tid * per + i).tiles;
-    int64_t upto = mine;
+    // ── this workgroup's item ── (each wave finds it for itself, a lane for every 64th of the
+    // requests: no barriers; ~1 us for up to 64)
+    const int per = (a.n_req + 63) >> 6;
+    const auto tiles_of = [&](int i) { return lane * per + i < a.n_req ? few_seg<KT>(a, lane * per + i).tiles : 0; };
+    const int tiles0 = tiles_of(0);
+    double mine = tiles0;
+    for (int i = 1; i < per; ++i) mine += tiles_of(i);
+    const int64_t U = (int64_t)pk_wave_sum_d(mine);             // (exact)
+    // The shortest chunk, from an equal share of U for each of W workgroups on, with which
+    // the items are at most W (give or take one for the division): all run at once, the
+    // longest of them for as little as such chunks allow. More requests than W: several rounds, of twice the share.
+    const int64_t share = max((U + W - 1) / W, (int64_t)FEW_WAVES);
+    int chunk = try_chunk(share, 6);
+    if (a.n_req <= W) {
+        float n[FEW_TRIES] = {};
+        for (int i = 0; i < per; ++i) {
+            const float tiles = (float)(i == 0 ? tiles0 : tiles_of(i));
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t u = __shfl_up(upto, d);
-        if (lane >= d) upto += u;
-    }
-    if (lane == 63) line[wave] = upto;
-    __syncthreads();
-    int64_t U = 0;
-    for (int w = 0; w < FEW_WAVES; ++w) {
-        if (w < wave) upto += line[w];
-        U += line[w];
-    }
-    if (U == 0) return;
-    // fewer workers than workgroups where the line is short: a tile for every wave
-    const int We = (int)min((int64_t)W, (U + FEW_WAVES - 1) / FEW_WAVES), w = blockIdx.x;
-    if (w >= We) return;
-    int64_t u0 = share(U, w, We);
-    const int64_t u1 = share(U, w + 1, We);
-    if (u0 >= upto - mine && u0 < upto) {
-        int64_t at = upto - mine;
-        int r = tid * per;
-        for (;; ++r) {
-            const int n = few_seg<KT>(a, r).tiles;
-            if (u0 < at + n) break;
-            at += n;
+            for (int k = 0; k < FEW_TRIES; ++k) n[k] += __builtin_ceilf(tiles * __builtin_amdgcn_rcpf((float)try_chunk(share, k)) * 0.999999f);
         }
-        start_r = r;
-        start_at = at;
+        int k = 0;
+#pragma unroll
+        for (int y = 0; y < FEW_TRIES - 1; ++y) k += k == y && pk_wave_sum_f(n[y]) > (float)W;
+        chunk = try_chunk(share, k);
     }
-    __syncthreads();
-    int r = start_r;
-    int64_t r_at = start_at;                                    // the request's first tile on the line
-
-    while (u0 < u1) {
-        const seg sg = few_seg<KT>(a, r);
-        if (sg.tiles == 0) { ++r; continue; }
-        const int t0 = (int)(u0 - r_at), t1 = (int)min(u1 - r_at, (int64_t)sg.tiles);
+    const auto items_of = [&](int tiles) { return (int)(((uint32_t)tiles + (uint32_t)chunk - 1) / (uint32_t)chunk); };
+    int items = 0, parts = 0;                                   // of this lane's requests; parts: of the split ones
+    for (int i = 0; i < per; ++i) {
+        const int n = items_of(i == 0 ? tiles0 : tiles_of(i));
+        items += n;
+        parts += n > 1 ? n : 0;
+    }
+    int at = wave_scan(items) - items, part_at = wave_scan(parts) - parts;
+    const uint64_t whose = __ballot((int)blockIdx.x >= at && (int)blockIdx.x < at + items);
+    if (whose == 0) return;
+    int my_r = 0, my_n = 0;
+    if (whose >> lane & 1)
+        for (int i = 0; i < per; ++i) {
+            my_n = items_of(i == 0 ? tiles0 : tiles_of(i));
+            my_r = lane * per + i;
+            if ((int)blockIdx.x < at + my_n) break;
+            at += my_n;
+            part_at += my_n > 1 ? my_n : 0;
+        }
+    const int src = __ffsll((unsigned long long)whose) - 1;
+    const int r = __builtin_amdgcn_readlane(my_r, src), n_it = __builtin_amdgcn_readlane(my_n, src);
+    const int it = (int)blockIdx.x - __builtin_amdgcn_readlane(at, src), part0 = __builtin_amdgcn_readlane(part_at, src);
+    const seg sg = few_seg<KT>(a, r);
+    const int t0 = (int)((int64_t)sg.tiles * it / n_it), t1 = (int)((int64_t)sg.tiles * (it + 1) / n_it);
+    {
         const int rows = min(sg.s.rows, min(a.max_q, COLS / G)), cols = rows * G;
         const int p_first = sg.s.kv - sg.s.rows, p_last = p_first + rows - 1;
         const int32_t *tab = a.table + (int64_t)r * a.max_blocks;
 
         // ── the queries: lane (m16, g) holds elements g KE .. of column m16 ──
         typedef typename regs<A, 8>::type q8;
-        q8 q[NQ][KV8];
+        c8 q[NQ][QP][KV8];
         int pos[NQ];
+        float scale2[NQ];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             const int c = n * 16 + m16, i = c / G;
             pos[n] = c < cols ? p_first + i : p_last;
             const A *src = (const A *)a.q + (int64_t)(sg.s.row0 + i) * a.q_stride + ((int64_t)kvh * G + (c - i * G)) * hd;
+            q8 v[KV8];
 #pragma unroll
             for (int s = 0; s < KV8; ++s) {
                 const int e = g * KE + 8 * s;
-                q[n][s] = q8{};
-                if (c < cols && e < hd) q[n][s] = *reinterpret_cast<const q8 *>(src + e);
+                v[s] = q8{};
+                if (c < cols && e < hd) v[s] = *reinterpret_cast<const q8 *>(src + e);
+            }
+            scale2[n] = a.scale2;
+            if constexpr (QP == 2) {                            // to a largest magnitude in [2^13, 2^14)
+                float top = 0.0f;
+#pragma unroll
+                for (int s = 0; s < KV8; ++s)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, __builtin_fabsf((float)v[s][i]));
+                top = pk_max_rows4(top);
+                const int k = min(max(14 - __builtin_amdgcn_frexp_expf(top), -114), 110);
+                const float up = __builtin_ldexpf(1.0f, k);
+#pragma unroll
+                for (int s = 0; s < KV8; ++s) v[s] *= up;
+                scale2[n] = a.scale2 * __builtin_ldexpf(1.0f, -k);
+            }
+#pragma unroll
+            for (int s = 0; s < KV8; ++s) {
+                c8 p[QP];
+                planes<C, QP>(v[s], p);
+#pragma unroll
+                for (int x = 0; x < QP; ++x) q[n][x][s] = p[x];
             }
         }
 
@@ -228,9 +309,10 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_attn_few(pk_attn_args a, flo
                     for (int n = 0; n < NQ; ++n) {
                         if constexpr (F32) {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) s[n][b] = mfma((float)k[b][x][e], q[n][x][e], s[n][b]);
+                            for (int e = 0; e < 8; ++e) s[n][b] = mfma(k[b][x][e], q[n][0][x][e], s[n][b]);
                         } else {
-                            s[n][b] = mfma(k[b][x], q[n][x], s[n][b]);
+#pragma unroll
+                            for (int y = 0; y < QP; ++y) s[n][b] = mfma(k[b][x], q[n][y][x], s[n][b]);
                         }
                     }
             const uint64_t ok_now = ok;
@@ -243,7 +325,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_attn_few(pk_attn_args a, flo
             // tiles that some row does not see whole
             const uint64_t all = KT == 64 ? ~0ull : (1ull << KT) - 1;
             const bool masked = (ok_now & all) != all || base + KT - 1 > p_first || (a.window > 0 && base <= p_last - a.window);
-            uint64_t odd = 0;                                   // keys with values that are not finite, seen by some rows only
+            uint64_t odd = 0;                                   // keys with values that are added one by one
             if (masked) {
                 // (the empty asm keeps this a branch: as selects it would be work of every tile)
                 uint64_t mine = ok_now >> (4 * g);
@@ -252,7 +334,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_attn_few(pk_attn_args a, flo
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int jj = b * 16 + 4 * g + i, j = base + jj;
+                        const int j = base + b * 16 + 4 * g + i;
                         const bool there = mine >> (b * 16 + i) & 1;
 #pragma unroll
                         for (int n = 0; n < NQ; ++n) {
@@ -260,18 +342,31 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_attn_few(pk_attn_args a, flo
                             if (!see) s[n][b][i] = -INFINITY;
                         }
                         const bool none = !there || j > p_last || (a.window > 0 && j <= p_first - a.window);
-                        const bool every = there && j <= p_first && (a.window <= 0 || j > p_last - a.window);
                         if (none) v[b][i] = vrow{};             // 0 x NaN
-                        bool bad = false;
-#pragma unroll
-                        for (int c = 0; c < VE; ++c) bad |= not_finite(v[b][i][c]);
-                        bad = bad && !every && VE * m16 < hd;
-                        const uint64_t who = __ballot(bad);     // (lanes of one g: one key)
-#pragma unroll
-                        for (int gg = 0; gg < 4; ++gg)
-                            if (who >> (16 * gg) & 0xffff) odd |= 1ull << (b * 16 + 4 * gg + i);
-                        if (odd >> jj & 1) v[b][i] = vrow{};
                     }
+            }
+            // Values that are not finite: with planes they meet zeros, and where some rows do not
+            // see them, zero probabilities.
+            if (masked || QP > 1) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) any |= odd_row<C, VE>(v[b][i]);
+                if (__any(any != 0 && VE * m16 < hd)) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int j = base + b * 16 + 4 * g + i;
+                            const bool every = j <= p_first && (a.window <= 0 || j > p_last - a.window);
+                            const uint64_t who = __ballot(odd_row<C, VE>(v[b][i]) != 0 && VE * m16 < hd && (QP > 1 || !every));
+#pragma unroll
+                            for (int gg = 0; gg < 4; ++gg)
+                                if (who >> (16 * gg) & 0xffff) odd |= 1ull << (b * 16 + 4 * gg + i);
+                            if (odd >> (b * 16 + 4 * g + i) & 1) v[b][i] = vrow{};
+                        }
+                }
             }
             // the running maximum, and probabilities in place of the scores
 #pragma unroll
@@ -281,7 +376,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_attn_few(pk_attn_args a, flo
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) top = fmaxf(top, s[n][b][i]);
-                top = pk_max_rows4(top) * a.scale2;
+                top = pk_max_rows4(top) * scale2[n] - SHIFT;
                 const float mn = fmaxf(mx[n], top);
                 // (nothing seen yet: any finite value keeps exp2 at 0)
                 const float ref = mn == -INFINITY ? 0.0f : mn, f = __builtin_amdgcn_exp2f(mx[n] - ref);
@@ -291,7 +386,7 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_attn_few(pk_attn_args a, flo
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][b][i], a.scale2, -ref));
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][b][i], scale2[n], -ref));
                         s[n][b][i] = p;
                         sum += p;
                     }
@@ -308,23 +403,27 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_attn_few(pk_attn_args a, flo
 #pragma unroll
                         for (int c = 0; c < VE; ++c)
 #pragma unroll
-                            for (int n = 0; n < NQ; ++n) o[n][c] = mfma((float)v[b][i][c], s[n][b][i], o[n][c]);
+                            for (int n = 0; n < NQ; ++n) o[n][c] = mfma(v[b][i][c], s[n][b][i], o[n][c]);
             } else {
-                typedef typename regs<A, 8>::type op8;
 #pragma unroll
                 for (int b = 0; b < NB; b += 2) {
-                    op8 p[NQ];
+                    c8 p[NQ][QP];
 #pragma unroll
-                    for (int n = 0; n < NQ; ++n)
+                    for (int n = 0; n < NQ; ++n) {
+                        typename regs<float, 8>::type x;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) p[n][i] = (A)s[n][b][i], p[n][4 + i] = (A)s[n][b + 1][i];
+                        for (int i = 0; i < 4; ++i) x[i] = s[n][b][i], x[4 + i] = s[n][b + 1][i];
+                        planes<C, QP>(x, p[n]);
+                    }
 #pragma unroll
                     for (int c = 0; c < VE; ++c) {
-                        op8 vt;
+                        c8 vt;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) vt[i] = v[b][i][c], vt[4 + i] = v[b + 1][i][c];
 #pragma unroll
-                        for (int n = 0; n < NQ; ++n) o[n][c] = mfma(vt, p[n], o[n][c]);
+                        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                            for (int x = 0; x < QP; ++x) o[n][c] = mfma(vt, p[n][x], o[n][c]);
                     }
                 }
             }
@@ -355,6 +454,17 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_attn_few(pk_attn_args a, flo
             }
         }
 
+        // a column's four elements from e on, and its lse
+        const auto finish = [&](const seg &sg, int kvh, int G, int c, int e, const f32x4 &acc, float l, float ref) {
+            const int i = c / G, h = kvh * G + (c - i * G);
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const int64_t row = sg.s.row0 + i;
+            typename regs<A, 4>::type v;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) v[z] = (A)(acc[z] * inv);
+            *reinterpret_cast<typename regs<A, 4>::type *>((A *)a.out + row * a.out_stride + (int64_t)h * hd + e) = v;
+            if (a.lse && e == 0) a.lse[row * a.H + h] = l == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * PK_LN2;
+        };
         // ── the waves' parts, joined ──
         __syncthreads();                                        // (so: the previous request's reads)
 #pragma unroll
@@ -368,9 +478,11 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_attn_few(pk_attn_args a, flo
                 for (int e = 0; e < VE; ++e) so[wave][c][VE * (4 * g + i) + e] = o[n][e][i];
         }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == sg.tiles;
+        const bool whole = n_it == 1;
         const int quads = hd >> 2;
-        float *slot = part + (((int64_t)kvh * W + w) * 2 + (t0 == 0)) * (COLS * (HDP + 4));
+        // a part: m and l of each column, then its sums
+        constexpr int PART = COLS * (HDP + 2);
+        float *first = part + ((int64_t)kvh * max_parts + part0) * PART, *slot = first + it * PART;
         for (int x = tid; x < cols * quads; x += FEW_THREADS) {
             const int c = x / quads, e = (x - c * quads) * 4;
             float mm = -INFINITY;
@@ -390,88 +502,105 @@ __global__ __launch_bounds__(FEW_THREADS, 2) void k_attn_few(pk_attn_args a, flo
                 for (int z = 0; z < 4; ++z) acc[z] = __builtin_fmaf(ov[z], f, acc[z]);
             }
             if (whole) {
-                l += __builtin_amdgcn_exp2f(sk - ref);
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const int64_t row = sg.s.row0 + i;
-                A *dst = (A *)a.out + row * a.out_stride + (int64_t)h * hd + e;
-                typename regs<A, 4>::type ov;
-#pragma unroll
-                for (int z = 0; z < 4; ++z) ov[z] = (A)(acc[z] * inv);
-                *reinterpret_cast<typename regs<A, 4>::type *>(dst) = ov;
-                if (a.lse && e == 0) a.lse[row * a.H + h] = l == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * PK_LN2;
+                finish(sg, kvh, G, c, e, acc, l + __builtin_amdgcn_exp2f(sk - ref), ref);
             } else {
-                float *p = slot + c * (HDP + 4);
                 const uint64_t *b = reinterpret_cast<const uint64_t *>(&acc);
+                uint64_t *p = (uint64_t *)(slot + 2 * COLS + c * HDP + e);
                 // past the L2: another XCD's workgroup may join
-                __hip_atomic_store((uint64_t *)(p + 4 + e), b[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store((uint64_t *)(p + 4 + e) + 1, b[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (e == 0) {
-                    __hip_atomic_store(p, mm, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    __hip_atomic_store(p + 1, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
+                __hip_atomic_store(p, b[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(p + 1, b[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (e == 0)
+                    __hip_atomic_store((uint64_t *)slot + c, (uint64_t)__float_as_uint(l) << 32 | __float_as_uint(mm), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
             }
         }
         if (!whole) {
-            // the request's parts: workers wa .. wb
-            const int wa = owner(r_at, U, We), wb = owner(r_at + sg.tiles - 1, U, We);
-            uint32_t *cnt = count + (int64_t)kvh * W + wa;
+            uint32_t *cnt = count + (int64_t)kvh * max_parts + part0;
             __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();
             if (tid == 0) {
                 const uint32_t was = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                last_in = was == (uint32_t)(wb - wa);
+                last_in = was == (uint32_t)(n_it - 1);
                 if (last_in) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             __syncthreads();
             if (last_in) {
-                const auto at = [&](int i, int c) {             // worker wa holds the request's start, the others its middle
-                    return part + (((int64_t)kvh * W + i) * 2 + (i == wa)) * (COLS * (HDP + 4)) + c * (HDP + 4);
-                };
-                const auto ld = [](const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-                for (int x = tid; x < cols * quads; x += FEW_THREADS) {
-                    const int c = x / quads, e = (x - c * quads) * 4;
-                    const int i = c / G, h = kvh * G + (c - i * G);
+                // (all loads past the L2)
+                const auto at = [&](int y) { return (const uint64_t *)(first + y * PART); };
+                const auto ld = [](const uint64_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+                const int np = n_it;
+                // references and sums: a wave per column, a lane per part
+                for (int c = wave; c < cols; c += FEW_WAVES) {
+                    const int h = kvh * G + c % G;
                     const float sk = a.sinks ? a.sinks[h] * PK_LOG2E : -INFINITY;
-                    float mm = sk;
-                    for (int y = wa; y <= wb; ++y) mm = fmaxf(mm, ld(at(y, c)));
-                    const float ref = mm == -INFINITY ? 0.0f : mm;
-                    float l = __builtin_amdgcn_exp2f(sk - ref);
-                    f32x4 acc = {0, 0, 0, 0};
-                    for (int y = wa; y <= wb; ++y) {
-                        const float *p = at(y, c);
-                        const float f = __builtin_amdgcn_exp2f(ld(p) - ref);
-                        l = __builtin_fmaf(ld(p + 1), f, l);
-                        uint64_t b[2];
-                        b[0] = __hip_atomic_load((const uint64_t *)(p + 4 + e), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                        b[1] = __hip_atomic_load((const uint64_t *)(p + 4 + e) + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                        const float *ov = reinterpret_cast<const float *>(b);
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) acc[z] = __builtin_fmaf(ov[z], f, acc[z]);
+                    float top = sk;
+                    for (int y = lane; y < np; y += 64) top = fmaxf(top, __uint_as_float((uint32_t)ld(at(y) + c)));
+                    top = pk_wave_max_f(top);
+                    const float ref = top == -INFINITY ? 0.0f : top;
+                    float l = lane == 0 ? __builtin_amdgcn_exp2f(sk - ref) : 0.0f;
+                    for (int y = lane; y < np; y += 64) {
+                        const uint64_t v = ld(at(y) + c);
+                        l = __builtin_fmaf(__uint_as_float((uint32_t)(v >> 32)), __builtin_amdgcn_exp2f(__uint_as_float((uint32_t)v) - ref), l);
                     }
-                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                    const int64_t row = sg.s.row0 + i;
-                    typename regs<A, 4>::type ov;
+                    l = pk_wave_sum_f(l);
+                    if (lane == 0) sm[0][c] = ref, sl[0][c] = l;
+                }
+                __syncthreads();
+                // the sums: four elements of a column per thread, the parts over as many groups of
+                // threads as there are, 8 of a group's parts in flight
+                const int items = cols * quads, groups = max(1, FEW_THREADS / items), grp = tid / items;
+                f32x4 *sums = reinterpret_cast<f32x4 *>(&so[0][0][0]);
+                for (int x = groups > 1 ? tid - grp * items : tid; x < items && grp < groups; x += FEW_THREADS) {
+                    const int c = x / quads, e = (x - c * quads) * 4;
+                    const float ref = sm[0][c];
+                    f32x4 acc = {0, 0, 0, 0};
+                    for (int y0 = grp; y0 < np; y0 += 8 * groups) {
+                        uint64_t m[8], v[8][2];
 #pragma unroll
-                    for (int z = 0; z < 4; ++z) ov[z] = (A)(acc[z] * inv);
-                    *reinterpret_cast<typename regs<A, 4>::type *>((A *)a.out + row * a.out_stride + (int64_t)h * hd + e) = ov;
-                    if (a.lse && e == 0)
-                        a.lse[row * a.H + h] = l == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * PK_LN2;
+                        for (int y = 0; y < 8; ++y) {
+                            const uint64_t *p = at(min(y0 + y * groups, np - 1));
+                            m[y] = ld(p + c);
+                            v[y][0] = ld(p + (2 * COLS + c * HDP + e) / 2);
+                            v[y][1] = ld(p + (2 * COLS + c * HDP + e) / 2 + 1);
+                        }
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) {
+                            const float f = y0 + y * groups < np ? __builtin_amdgcn_exp2f(__uint_as_float((uint32_t)m[y]) - ref) : 0.0f;
+                            if (f == 0.0f) continue;
+                            const float *ov = reinterpret_cast<const float *>(v[y]);
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) acc[z] = __builtin_fmaf(ov[z], f, acc[z]);
+                        }
+                    }
+                    if (groups > 1) sums[tid] = acc;
+                    else finish(sg, kvh, G, c, e, acc, sl[0][c], ref);
+                }
+                if (groups > 1) {
+                    __syncthreads();
+                    if (tid < items) {
+                        f32x4 acc = sums[tid];
+                        for (int y = 1; y < groups; ++y)
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) acc[z] += sums[y * items + tid][z];
+                        const int c = tid / quads;
+                        finish(sg, kvh, G, c, (tid - c * quads) * 4, acc, sl[0][c], sm[0][c]);
+                    }
                 }
             }
         }
-        u0 = r_at + t1;
-        r_at += sg.tiles;
-        ++r;
     }
 }
 
 template <typename A, typename C, int HDP, int NQ>
 int launch(pk_engine *e, const pk_attn_args &a, int64_t tiles) {
-    // workers per KV head: two workgroups per CU in all, no more than the line may have tiles for its waves
-    const int64_t most = (tiles + FEW_WAVES - 1) / FEW_WAVES;
-    const int W = (int)std::max<int64_t>(1, std::min<int64_t>(most, (2 * e->n_cu + a.KVH - 1) / a.KVH));
-    PK_TRY(pk_attn_workspace(e, (int64_t)a.KVH * W * 2 * 16 * NQ * (HDP + 4), (int64_t)a.KVH * W));
-    k_attn_few<A, C, HDP, NQ><<<dim3((unsigned)W, (unsigned)a.KVH), FEW_THREADS, 0, e->stream>>>(a, e->att_ws, e->att_cnt);
+    // W: two workgroups on every CU. The items are at most W chunks and one for each request,
+    // and never more than the tiles; the split requests' parts at most 2 W, since each of them is
+    // longer than a chunk
+    const int64_t slots = (FEW_PER_CU * (int64_t)e->n_cu + a.KVH - 1) / a.KVH;
+    const int W = (int)std::max<int64_t>(slots, 1);
+    const int64_t grid = std::min<int64_t>(W + (int64_t)a.n_req, std::max<int64_t>(tiles, 1));
+    PK_TRY(pk_attn_workspace(e, (int64_t)a.KVH * 2 * W * 16 * NQ * (HDP + 2), (int64_t)a.KVH * 2 * W));
+    k_attn_few<A, C, HDP, NQ><<<dim3((unsigned)grid, (unsigned)a.KVH), FEW_THREADS, 0, e->stream>>>(a, W, 2 * W, e->att_ws, e->att_cnt);
     PK_HIP(hipGetLastError());
     return PK_OK;
 }
@@ -487,9 +616,10 @@ int by_shape(pk_engine *e, const pk_attn_args &a, int64_t positions) {
 
 }  // namespace
 
-int pk_launch_attn_few(pk_engine *e, const pk_attn_args &a, int max_kv) {
-    // (with a window, a row reads no more than it and a tile's rest)
-    const int64_t positions = a.window > 0 ? std::min<int64_t>(max_kv, (int64_t)a.window + a.max_q + 64) : max_kv;
+int pk_launch_attn_few(pk_engine *e, const pk_attn_args &a) {
+    // positions that a request's rows may read: its table's, or a window and a tile's rest
+    const int64_t cap = (int64_t)a.max_blocks << a.page_shift;
+    const int64_t positions = a.window > 0 ? std::min<int64_t>(cap, (int64_t)a.window + a.max_q + 64) : cap;
 #define PK_FEW(A, C) return by_shape<A, C>(e, a, positions)
     PK_BY_TYPES(a.type, a.cache_type, PK_FEW);
 #undef PK_FEW
