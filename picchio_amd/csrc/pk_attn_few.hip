@@ -96,7 +96,7 @@ __device__ __forceinline__ seg few_seg(const pk_attn_args &a, int r) {
     return g;
 }
 
-constexpr int FEW_TRIES = 8;
+constexpr int FEW_TRIES = 8, FEW_KEPT = 4;
 __device__ __forceinline__ int try_chunk(int64_t share, int k) {
     return (int)min(share + share * (k < 5 ? k : 2 * k - 4) / 8, (int64_t)INT32_MAX / 2);     // 1, 9/8 .. 12/8, 14/8, 2, 18/8
 }
@@ -133,59 +133,93 @@ __global__ __launch_bounds__(FEW_THREADS, FEW_PER_CU) void k_attn_few(pk_attn_ar
 
     __shared__ __attribute__((aligned(16))) float so[FEW_WAVES][COLS][LD];
     __shared__ float sm[FEW_WAVES][COLS], sl[FEW_WAVES][COLS];
-    __shared__ int last_in;
+    __shared__ double wave_tiles[FEW_WAVES];
+    __shared__ int wave_items[FEW_WAVES][2], found[4], last_in;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m16 = lane & 15;
     const int kvh = blockIdx.y, G = a.H / a.KVH, hd = a.hd;
     const int ps = 1 << a.page_shift;
 
-    // ── this workgroup's item ── (each wave finds it for itself, a lane for every 64th of the
-    // requests: no barriers; ~1 us for up to 64)
-    const int per = (a.n_req + 63) >> 6;
-    const auto tiles_of = [&](int i) { return lane * per + i < a.n_req ? few_seg<KT>(a, lane * per + i).tiles : 0; };
-    const int tiles0 = tiles_of(0);
-    double mine = tiles0;
-    for (int i = 1; i < per; ++i) mine += tiles_of(i);
-    const int64_t U = (int64_t)pk_wave_sum_d(mine);             // (exact)
-    // The shortest chunk, from an equal share of U for each of W workgroups on, with which
-    // the items are at most W (give or take one for the division): all run at once, the
-    // longest of them for as little as such chunks allow. More requests than W: several rounds, of twice the share.
-    const int64_t share = max((U + W - 1) / W, (int64_t)FEW_WAVES);
-    int chunk = try_chunk(share, 6);
-    if (a.n_req <= W) {
-        float n[FEW_TRIES] = {};
-        for (int i = 0; i < per; ++i) {
-            const float tiles = (float)(i == 0 ? tiles0 : tiles_of(i));
+    // ── this workgroup's item ──
+    // Up to 64 FEW_KEPT requests: each wave finds it for itself, a lane for every 64th of the
+    // requests, with no barriers (~1 us). More: a thread for every 256th.
+    const bool wide = a.n_req > 64 * FEW_KEPT;
+    const int id = wide ? tid : lane, per = wide ? (a.n_req + FEW_THREADS - 1) / FEW_THREADS : (a.n_req + 63) >> 6;
+    const auto tiles_of = [&](int i) { return i < per && id * per + i < a.n_req ? few_seg<KT>(a, id * per + i).tiles : 0; };
+    int tiles[FEW_KEPT];                                        // (the first FEW_KEPT of a lane: read once)
 #pragma unroll
-            for (int k = 0; k < FEW_TRIES; ++k) n[k] += __builtin_ceilf(tiles * __builtin_amdgcn_rcpf((float)try_chunk(share, k)) * 0.999999f);
-        }
+    for (int i = 0; i < FEW_KEPT; ++i) tiles[i] = tiles_of(i);
+    const auto each = [&](auto f) {                             // f(i, tiles) in order, until it is true
+#pragma unroll
+        for (int i = 0; i < FEW_KEPT; ++i)
+            if (i < per && f(i, tiles[i])) return;
+        for (int i = FEW_KEPT; i < per; ++i)
+            if (f(i, tiles_of(i))) return;
+    };
+    double all = 0.0;
+    each([&](int, int n) { all += n; return false; });
+    all = pk_wave_sum_d(all);                                   // (exact)
+    if (wide) {
+        if (lane == 0) wave_tiles[wave] = all;
+        __syncthreads();
+        all = wave_tiles[0] + wave_tiles[1] + wave_tiles[2] + wave_tiles[3];
+    }
+    // The shortest chunk, from an equal share of the tiles for each of W workgroups on, with which
+    // the items are at most W (give or take one for the division): all run at once, the
+    // longest of them for as little as such chunks allow. More requests than W (or than
+    // are worth the search): several rounds, of twice the share.
+    const int64_t share = max(((int64_t)all + W - 1) / W, (int64_t)FEW_WAVES);
+    int chunk = try_chunk(share, 6);
+    if (a.n_req <= W && !wide) {
+        float n[FEW_TRIES] = {};
+        each([&](int, int t) {
+#pragma unroll
+            for (int k = 0; k < FEW_TRIES; ++k) n[k] += __builtin_ceilf((float)t * __builtin_amdgcn_rcpf((float)try_chunk(share, k)) * 0.999999f);
+            return false;
+        });
         int k = 0;
 #pragma unroll
         for (int y = 0; y < FEW_TRIES - 1; ++y) k += k == y && pk_wave_sum_f(n[y]) > (float)W;
         chunk = try_chunk(share, k);
     }
-    const auto items_of = [&](int tiles) { return (int)(((uint32_t)tiles + (uint32_t)chunk - 1) / (uint32_t)chunk); };
+    const auto items_of = [&](int t) { return (int)(((uint32_t)t + (uint32_t)chunk - 1) / (uint32_t)chunk); };
     int items = 0, parts = 0;                                   // of this lane's requests; parts: of the split ones
-    for (int i = 0; i < per; ++i) {
-        const int n = items_of(i == 0 ? tiles0 : tiles_of(i));
+    each([&](int, int t) {
+        const int n = items_of(t);
         items += n;
         parts += n > 1 ? n : 0;
+        return false;
+    });
+    int at = wave_scan(items), part_at = wave_scan(parts);
+    if (wide) {
+        if (lane == 63) wave_items[wave][0] = at, wave_items[wave][1] = part_at;
+        if (tid == 0) found[0] = -1;
+        __syncthreads();
+        for (int i = 0; i < wave; ++i) at += wave_items[i][0], part_at += wave_items[i][1];
     }
-    int at = wave_scan(items) - items, part_at = wave_scan(parts) - parts;
+    at -= items;
+    part_at -= parts;
     const uint64_t whose = __ballot((int)blockIdx.x >= at && (int)blockIdx.x < at + items);
-    if (whose == 0) return;
     int my_r = 0, my_n = 0;
     if (whose >> lane & 1)
-        for (int i = 0; i < per; ++i) {
-            my_n = items_of(i == 0 ? tiles0 : tiles_of(i));
-            my_r = lane * per + i;
-            if ((int)blockIdx.x < at + my_n) break;
+        each([&](int i, int t) {
+            my_n = items_of(t);
+            my_r = id * per + i;
+            if ((int)blockIdx.x < at + my_n) return true;
             at += my_n;
             part_at += my_n > 1 ? my_n : 0;
-        }
-    const int src = __ffsll((unsigned long long)whose) - 1;
-    const int r = __builtin_amdgcn_readlane(my_r, src), n_it = __builtin_amdgcn_readlane(my_n, src);
-    const int it = (int)blockIdx.x - __builtin_amdgcn_readlane(at, src), part0 = __builtin_amdgcn_readlane(part_at, src);
+            return false;
+        });
+    const int src = whose ? __ffsll((unsigned long long)whose) - 1 : 0;
+    int r = whose ? __builtin_amdgcn_readlane(my_r, src) : -1, n_it = __builtin_amdgcn_readlane(my_n, src);
+    int it = (int)blockIdx.x - __builtin_amdgcn_readlane(at, src), part0 = __builtin_amdgcn_readlane(part_at, src);
+    if (wide) {
+        if (whose && lane == 0) found[0] = r, found[1] = n_it, found[2] = it, found[3] = part0;
+        __syncthreads();
+        r = __builtin_amdgcn_readfirstlane(found[0]), n_it = __builtin_amdgcn_readfirstlane(found[1]);
+        it = __builtin_amdgcn_readfirstlane(found[2]), part0 = __builtin_amdgcn_readfirstlane(found[3]);
+    }
+    if (r < 0) return;
     const seg sg = few_seg<KT>(a, r);
     const int t0 = (int)((int64_t)sg.tiles * it / n_it), t1 = (int)((int64_t)sg.tiles * (it + 1) / n_it);
     {

@@ -373,3 +373,33 @@ def test_same_bits_again(eng, dtype):
         seen.append([x.clone() for x in (p.out, p.lse, g.out, g.lse)])
     for s in seen[1:]:
         assert all(torch.equal(x, y) for x, y in zip(s, seen[0]))
+
+
+@pytest.mark.parametrize("n", [64, 65, 200, 256, 257, 1000])
+def test_paged_many_requests(eng, n):
+    """More requests than a wave's lanes or a workgroup finds at once: some idle,
+    one far longer than the others, some of several rows."""
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    kv = [1 + (37 * i) % 150 for i in range(n)]
+    q = [0 if i % 7 == 3 else min(k, 1 + (i % 11 == 5)) for i, k in enumerate(kv)]
+    kv[n // 3] = 6000
+    p = Paged(gen, q, kv, 8, 2, 64, BF16, BF16, 16)
+    p.run(eng)
+    p.verify()
+
+
+@pytest.mark.parametrize("act,cache", [(F32, F16), (F32, BF16), (F16, F16)])
+def test_paged_magnitudes(eng, act, cache):
+    """Queries from 2^-40 to 2^40 in rows of one call, over keys that bring the
+    scores back to around 1 (fp32 queries over a 16-bit cache are scaled and cut
+    into planes); values at the ends of the cache's type."""
+    gen = torch.Generator(device="cuda").manual_seed(14)
+    p = Paged(gen, [1] * 5, [300] * 5, 8, 2, 64, act, cache, 16)
+    e = [-40, -20, 0, 20, 40] if act == F32 and cache == BF16 else [-12, -6, 0, 6, 10]
+    for r in range(5):
+        p.q[r] *= 2.0 ** e[r]
+        p.k[r] *= 2.0 ** -e[r]
+        p.v[r] *= 2.0 ** (10 if cache == F16 else 60) if r % 2 else 2.0 ** (-10 if cache == F16 else -60)
+    p.fill()
+    p.run(eng)
+    p.verify()
