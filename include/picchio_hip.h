@@ -460,7 +460,7 @@ typedef struct pk_pages {
 
 /* Free pages are kept in a ring of n_pages entries: ring_state_dev[0] is the
  * place of the first, [1] their number (at the start: 0 and n_pages, the ring
- * holding every page id once), [2] and [3] the library's (0 at the start).
+ * holding every page id once); [2] and [3] are not used.
  * For request r with lengths old_len_dev[r] and new_len_dev[r] in positions
  * (cut to 0 .. max_blocks * page_size), in order of r:
  *  - a request that grows gets ceil(new / page_size) - ceil(old / page_size)

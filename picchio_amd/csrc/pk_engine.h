@@ -45,7 +45,8 @@ constexpr int PK_CTR_POLL_BOUND = 41;    // their bound on polls per wait (0: th
 constexpr int PK_CTR_COMBINE = 64;        // [row blocks] down+combine arrivals
 constexpr int PK_CTR_ATTN = 4096;         // [rows x heads] attention chunk arrivals
 constexpr int PK_CTR_ATTN_N = 4096;
-constexpr int PK_CTR_N = PK_CTR_ATTN + PK_CTR_ATTN_N;
+constexpr int PK_CTR_PLAN = PK_CTR_ATTN + PK_CTR_ATTN_N;   // [17][16] k_plan_pages arrivals, a word of each 64 bytes
+constexpr int PK_CTR_N = PK_CTR_PLAN + 17 * 16;
 
 // Sets of launches that a decode step's draw is made of (pk_step_key).
 constexpr int PK_STEPS = 8;

@@ -45,111 +45,163 @@ int pk_check_rows(const void *p, int64_t stride, int heads, int hd, const char *
 namespace {
 
 // ───────────────────────── pages of a step ─────────────────────────
-// One launch. Every workgroup adds up the requests' pages and rows for itself
-// (three running sums over at most 4096 requests, ~1 us) and keeps the row
-// starts and page places in LDS; then it moves the pages of its share of the
-// requests and writes its share of the rows. Two launches, sums first, would
-// save the repeated sums but cost a launch more than those. What a
-// workgroup reads of the table and the ring (pages below ceil(old / page_size);
-// the ring's free entries) no other one writes; the ring's state is
-// written by the workgroup that arrives last, when all have read it.
-constexpr int PLAN_THREADS = 512, PLAN_REQ = 4096, PLAN_PER = PLAN_REQ / PLAN_THREADS;
+// One launch: bound by its latency (a step of 32 requests 6.7 us) and, for long
+// prompts, by the write of the rows. Every workgroup adds up the requests' pages
+// and rows for itself (three running sums over at most 4096 requests, ~1 us) and
+// keeps row starts, page places and old lengths in LDS; then it moves the pages of
+// its share of the requests and writes its share of the rows, four neighbours per
+// thread, which find their request once and write 16 bytes (1000 requests, 1.3 M
+// rows: 12.6 us, one row per thread 15.3). Two launches, sums first, would save the
+// repeated sums but cost a launch more than those. What a workgroup reads of the
+// table and the ring (pages below ceil(old / page_size); the ring's free entries)
+// no other one writes; the ring's state is written by the workgroup that arrives
+// last, when all have read it.
+constexpr int PLAN_THREADS = 512, PLAN_REQ = 4096, PLAN_PER = PLAN_REQ / PLAN_THREADS, PLAN_ROWS = 4 * PLAN_THREADS;
 
-// Inclusive sums of v over the block (PLAN_THREADS threads).
+// Sums that stay at 2^31 - 1 once they would pass it (more than any count they are
+// compared with).
+__device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, 0x7fffffffu); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_sat_add(uint32_t v) {
+    return sat_add(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, true));
+}
+// Sums over the block's threads up to this one.
 template <int N>
-__device__ __forceinline__ void block_sums(int64_t (&v)[N], int64_t (*part)[N]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__device__ __forceinline__ void block_sums(uint32_t (&v)[N], uint32_t (*part)[N]) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1)
+    for (int k = 0; k < N; ++k) {
+        v[k] = dpp_sat_add<0x111, 0xf>(v[k]);                  // row_shr 1, 2, 4, 8
+        v[k] = dpp_sat_add<0x112, 0xf>(v[k]);
+        v[k] = dpp_sat_add<0x114, 0xf>(v[k]);
+        v[k] = dpp_sat_add<0x118, 0xf>(v[k]);
+        v[k] = dpp_sat_add<0x142, 0xa>(v[k]);                  // lane 15 of a row to the next row, 31 to the upper half
+        v[k] = dpp_sat_add<0x143, 0xc>(v[k]);
+    }
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 63)
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int64_t u = __shfl_up(v[k], d);
-            if (lane >= d) v[k] += u;
-        }
-    if (lane == 63)
         for (int k = 0; k < N; ++k) part[wave][k] = v[k];
     __syncthreads();
-    for (int w = 0; w < wave; ++w)
-        for (int k = 0; k < N; ++k) v[k] += part[w][k];
+#pragma unroll
+    for (int w = 0; w < PLAN_THREADS / 64; ++w)
+        if (w < wave)
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] = sat_add(v[k], part[w][k]);
 }
 
 __global__ __launch_bounds__(PLAN_THREADS) void k_plan_pages(
     int n_req, int max_blocks, int n_pages, int shift, int max_tokens, const int32_t *__restrict__ old_len,
     const int32_t *__restrict__ new_len, int32_t *table, int32_t *ring, int32_t *state, int32_t *len, int32_t *cu_q,
-    int32_t *__restrict__ slot, int32_t *__restrict__ pos) {
-    __shared__ int32_t cu[PLAN_REQ + 1], place[PLAN_REQ];       // row starts; ring offsets of a request's pages
-    __shared__ int64_t part[PLAN_THREADS / 64][3];
+    int32_t *__restrict__ slot, int32_t *__restrict__ pos, uint32_t *arrivals) {
+    __shared__ int32_t cu[PLAN_REQ + 1], place[PLAN_REQ], old[PLAN_REQ];    // row starts; ring places of pages; old lengths
+    __shared__ uint32_t part[PLAN_THREADS / 64][3];
     __shared__ int32_t stop, moved[2];                          // first request not served; pages taken, given
     const int t = threadIdx.x, most = max_blocks << shift, up = (1 << shift) - 1;
-    const int head = (int)(((int64_t)state[0] % n_pages + n_pages) % n_pages);
     const int count = min(max(state[1], 0), n_pages);
+    const int head = (int)((uint32_t)state[0] % (uint32_t)n_pages);
     if (t == 0) stop = n_req;
     // a thread's requests are neighbours
     const int per = (n_req + PLAN_THREADS - 1) / PLAN_THREADS, r0 = t * per;
-    int64_t sum[3] = {0, 0, 0};                                 // pages taken, rows, pages given
+    uint32_t sum[3] = {0, 0, 0};                                // pages taken, rows, pages given
     int a[PLAN_PER], b[PLAN_PER];
 #pragma unroll
     for (int i = 0; i < PLAN_PER; ++i) {
         a[i] = b[i] = 0;
-        if (i < per && r0 + i < n_req) {
+        if (i >= per) break;
+        if (r0 + i < n_req) {
             a[i] = min(max(old_len[r0 + i], 0), most);
             b[i] = min(max(new_len[r0 + i], 0), most);
         }
         const int d = ((b[i] + up) >> shift) - ((a[i] + up) >> shift);
-        sum[0] += max(d, 0);
-        sum[1] += max(b[i] - a[i], 0);
-        sum[2] += max(-d, 0);
+        sum[0] = sat_add(sum[0], max(d, 0));
+        sum[1] = sat_add(sum[1], max(b[i] - a[i], 0));
+        sum[2] = sat_add(sum[2], max(-d, 0));
     }
-    int64_t at[3] = {sum[0], sum[1], sum[2]};
+    // sums before this thread's requests: those up to the thread before
+    uint32_t at[3] = {sum[0], sum[1], sum[2]};
     block_sums(at, part);                                       // (its barrier also covers `stop`)
+    uint32_t at0[3];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) at[k] -= sum[k];
-    const int64_t at0[3] = {at[0], at[1], at[2]};
+    for (int k = 0; k < 3; ++k) {
+        at0[k] = (uint32_t)__shfl_up((int)at[k], 1);
+        if ((t & 63) == 0) {
+            at0[k] = 0;
+            for (int w = 0; w < t >> 6; ++w) at0[k] = sat_add(at0[k], part[w][k]);
+        }
+        at[k] = at0[k];
+    }
     // the sums only grow: from the first request that does not fit on, none that grows does
 #pragma unroll
     for (int i = 0; i < PLAN_PER; ++i) {
+        if (i >= per) break;
         const int d = ((b[i] + up) >> shift) - ((a[i] + up) >> shift);
-        at[0] += max(d, 0);
-        at[1] += max(b[i] - a[i], 0);
-        if (i < per && r0 + i < n_req && (at[0] > count || at[1] > max_tokens)) atomicMin(&stop, r0 + i);
+        at[0] = sat_add(at[0], max(d, 0));
+        at[1] = sat_add(at[1], max(b[i] - a[i], 0));
+        if (r0 + i < n_req && (at[0] > (uint32_t)count || at[1] > (uint32_t)max_tokens)) atomicMin(&stop, r0 + i);
     }
     __syncthreads();
     const int last = stop;
-    at[0] = at0[0], at[1] = at0[1], at[2] = at0[2];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) at[k] = at0[k];
 #pragma unroll
     for (int i = 0; i < PLAN_PER; ++i) {
         const int r = r0 + i;
-        if (i >= per || r >= n_req) continue;
+        if (i >= per) break;
+        if (r >= n_req) continue;
+        old[r] = a[i];
         if (r <= last) cu[r] = (int32_t)at[1];
         if (r == last) moved[0] = (int32_t)at[0];
         const int d = ((b[i] + up) >> shift) - ((a[i] + up) >> shift);
-        place[r] = d < 0 ? (int32_t)((count + at[2]) % n_pages) : (int32_t)min(at[0], (int64_t)n_pages);
-        at[0] += max(d, 0);
-        at[1] += max(b[i] - a[i], 0);
-        at[2] += max(-d, 0);
+        // (served requests' pages are at most `count` from the head; head, count < 2^28)
+        const uint32_t x = (uint32_t)head + (d < 0 ? (uint32_t)count + at[2] : min(at[0], (uint32_t)count));
+        place[r] = (int32_t)(x % (uint32_t)n_pages);
+        at[0] = sat_add(at[0], max(d, 0));
+        at[1] = sat_add(at[1], max(b[i] - a[i], 0));
+        at[2] = sat_add(at[2], max(-d, 0));
         if (r == n_req - 1) {
             if (last == n_req) cu[n_req] = (int32_t)at[1], moved[0] = (int32_t)at[0];
-            moved[1] = (int32_t)min(at[2], (int64_t)n_pages);
+            moved[1] = (int32_t)min(at[2], (uint32_t)n_pages);
         }
     }
     if (n_req == 0 && t == 0) cu[0] = moved[0] = moved[1] = 0;
     __syncthreads();
     // (requests behind the last one served have no rows)
-    for (int r = last + 1 + t; r <= n_req; r += PLAN_THREADS) cu[r] = cu[last];
-    __syncthreads();
+    if (last < n_req) {
+        for (int r = last + 1 + t; r <= n_req; r += PLAN_THREADS) cu[r] = cu[last];
+        __syncthreads();
+    }
+    // The state is read; the last workgroup to have done so writes it. Arrivals in two
+    // steps, 16 words and then one (650 on one word take 10 us), by a wave while the others go on.
+    if (t == PLAN_THREADS - 64) {
+        const auto arrive = [&](uint32_t *c, uint32_t of) {
+            const bool last_in = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == of;
+            if (last_in) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            return last_in;
+        };
+        const uint32_t group = blockIdx.x & 15, groups = min(gridDim.x, 16u);
+        if (arrive(arrivals + 16 * (1 + group), (gridDim.x + 15 - group) >> 4) && arrive(arrivals, groups)) {
+            state[0] = (int32_t)(((uint32_t)head + (uint32_t)moved[0]) % (uint32_t)n_pages);
+            state[1] = min(count - moved[0] + moved[1], n_pages);
+        }
+    }
+    // entry k of the ring from a place on (k < n_pages)
+    const auto from = [&](int place, int k) {
+        const uint32_t x = (uint32_t)place + (uint32_t)k;
+        return x >= (uint32_t)n_pages ? x - (uint32_t)n_pages : x;
+    };
 
     // the pages: a wave per request
     const int lane = t & 63, waves = gridDim.x * (PLAN_THREADS / 64);
     for (int r = blockIdx.x * (PLAN_THREADS / 64) + (t >> 6); r < n_req; r += waves) {
-        const int o = min(max(old_len[r], 0), most), n = min(max(new_len[r], 0), most);
+        const int o = old[r], n = min(max(new_len[r], 0), most);
         const int ob = (o + up) >> shift, nb = (n + up) >> shift;
         int32_t *row = table + (int64_t)r * max_blocks;
         if (n > o) {
             if (r < last)
-                for (int k = ob + lane; k < nb; k += 64) row[k] = ring[((int64_t)head + place[r] + (k - ob)) % n_pages];
+                for (int k = ob + lane; k < nb; k += 64) row[k] = ring[from(place[r], k - ob)];
         } else {
             for (int k = nb + lane; k < ob; k += 64) {
-                ring[((int64_t)head + place[r] + (k - nb)) % n_pages] = row[k];
+                ring[((uint32_t)place[r] + (uint32_t)(k - nb)) % (uint32_t)n_pages] = row[k];
                 row[k] = -1;
             }
         }
@@ -162,31 +214,48 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_plan_pages(
 
     // the rows
     const int total = cu[n_req];
-    for (int64_t i = (int64_t)blockIdx.x * PLAN_THREADS + t; i < max_tokens; i += (int64_t)gridDim.x * PLAN_THREADS) {
-        int p = 0, s = -1;
-        if (i < total) {
-            int lo = 0, hi = n_req - 1;                         // the last request that starts at or before row i
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (cu[mid] <= (int)i) lo = mid;
-                else hi = mid - 1;
-            }
-            const int o = min(max(old_len[lo], 0), most), ob = (o + up) >> shift;
-            p = o + ((int)i - cu[lo]);
-            const int k = p >> shift;
-            const int page = k < ob ? table[(int64_t)lo * max_blocks + k]
-                                    : ring[((int64_t)head + place[lo] + (k - ob)) % n_pages];
-            if (page >= 0 && page < n_pages) s = (page << shift) + (p & up);
+    const bool wide = (((uintptr_t)slot | (uintptr_t)pos) & 15) == 0;
+    // the last of the requests lo .. hi that starts at or before row i
+    const auto find = [&](int i, int lo, int hi) {
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (cu[mid] <= i) lo = mid;
+            else hi = mid - 1;
         }
-        slot[i] = s;
-        pos[i] = p;
-    }
-    if (t == 0) {
-        const uint32_t was = __hip_atomic_fetch_add((uint32_t *)state + 2, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (was + 1 == gridDim.x) {
-            state[0] = (int32_t)(((int64_t)head + moved[0]) % n_pages);
-            state[1] = min(count - moved[0] + moved[1], n_pages);
-            state[2] = 0;
+        return lo;
+    };
+    for (int64_t base = (int64_t)blockIdx.x * PLAN_ROWS; base < max_tokens; base += (int64_t)gridDim.x * PLAN_ROWS) {
+        const int64_t i0 = base + t * 4;
+        int p[4], s[4];
+        int r = -1, end = 0, off = 0, ob = 0, k_at = -1, page = -1;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int64_t i = i0 + q;
+            p[q] = 0, s[q] = -1;
+            if (i >= total) continue;
+            if (r < 0 || i >= end) {
+                r = find((int)i, r + 1, n_req - 1);
+                end = cu[r + 1];
+                const int o = old[r];
+                off = o - cu[r];
+                ob = (o + up) >> shift;
+                k_at = -1;
+            }
+            p[q] = off + (int)i;
+            const int k = p[q] >> shift;
+            if (k != k_at) {
+                k_at = k;
+                page = k < ob ? table[(int64_t)r * max_blocks + k] : ring[from(place[r], k - ob)];
+            }
+            if (page >= 0 && page < n_pages) s[q] = (page << shift) + (p[q] & up);
+        }
+        if (wide && i0 + 3 < max_tokens) {
+            *reinterpret_cast<int4 *>(slot + i0) = int4{s[0], s[1], s[2], s[3]};
+            *reinterpret_cast<int4 *>(pos + i0) = int4{p[0], p[1], p[2], p[3]};
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (i0 + q < max_tokens) slot[i0 + q] = s[q], pos[i0 + q] = p[q];
         }
     }
 }
@@ -263,10 +332,12 @@ extern "C" int pk_plan_pages(pk_engine *e, const pk_page_plan *p) {
              PK_ERR_ARG, "plan_pages: len_dev overlaps new_len_dev");
     pk_device_scope dev(e->device);
     PK_TRY(dev.rc);
-    const int64_t wgs = std::max<int64_t>(((int64_t)p->max_tokens + PLAN_THREADS - 1) / PLAN_THREADS, (p->n_req + 31) / 32);
-    k_plan_pages<<<(unsigned)std::min<int64_t>(std::max<int64_t>(wgs, 1), 512), PLAN_THREADS, 0, e->stream>>>(
+    // (three workgroups per CU at most: 256 to 1024 of them measured alike)
+    const int64_t wgs = std::max<int64_t>(((int64_t)p->max_tokens + PLAN_ROWS - 1) / PLAN_ROWS, (p->n_req + 31) / 32);
+    k_plan_pages<<<(unsigned)std::min<int64_t>(std::max<int64_t>(wgs, 1), 768), PLAN_THREADS, 0, e->stream>>>(
         p->n_req, p->max_blocks, p->n_pages, __builtin_ctz((unsigned)p->page_size), p->max_tokens, p->old_len_dev,
-        p->new_len_dev, p->table_dev, p->ring_dev, p->ring_state_dev, p->len_dev, p->cu_q_dev, p->slot_dev, p->pos_dev);
+        p->new_len_dev, p->table_dev, p->ring_dev, p->ring_state_dev, p->len_dev, p->cu_q_dev, p->slot_dev, p->pos_dev,
+        e->counters + PK_CTR_PLAN);
     PK_HIP(hipGetLastError());
     return PK_OK;
 }
