@@ -84,7 +84,7 @@ __device__ __forceinline__ uint32_t odd_row(const typename regs<T, N>::type &v) 
 // A request's tiles.
 struct seg {
     pk_span s;
-    int first, tiles;          // first position (a multiple of KT), tiles (0: no rows; at least 1 otherwise)
+    int first, end, tiles;     // first position (a multiple of KT), the one behind the last, tiles (0: no rows; at least 1 otherwise)
 };
 template <int KT>
 __device__ __forceinline__ seg few_seg(const pk_attn_args &a, int r) {
@@ -92,7 +92,8 @@ __device__ __forceinline__ seg few_seg(const pk_attn_args &a, int r) {
     g.s = pk_request(a, r);
     const int p0 = max(g.s.kv - g.s.rows, 0);                  // the first row's position
     g.first = a.window > 0 ? max(p0 - a.window + 1, 0) & ~(KT - 1) : 0;
-    g.tiles = g.s.rows && !(a.few_only && g.s.rows > a.max_q) ? max((g.s.kv - g.first + KT - 1) / KT, 1) : 0;
+    g.end = max(g.s.kv - max(g.s.rows - a.max_q, 0), 0);       // (rows beyond max_q are not computed: nor their positions read)
+    g.tiles = g.s.rows && !(a.few_only && g.s.rows > a.max_q) ? max((g.end - g.first + KT - 1) / KT, 1) : 0;
     return g;
 }
 
@@ -280,8 +281,8 @@ __global__ __launch_bounds__(FEW_THREADS, FEW_PER_CU) void k_attn_few(pk_attn_ar
         // Page of position j (a position past the end or a page that is none: page 0, and the bit of j not set)
         const auto look = [&](int t, uint64_t &ok) {
             const int j = sg.first + t * KT + (lane & (KT - 1));
-            const int pg = tab[min(j, max(sg.s.kv - 1, 0)) >> a.page_shift];
-            const bool good = j < sg.s.kv && pg >= 0 && pg < a.n_pages;
+            const int pg = tab[min(j, max(sg.end - 1, 0)) >> a.page_shift];
+            const bool good = j < sg.end && pg >= 0 && pg < a.n_pages;
             ok = __ballot(good);
             return good ? pg : 0;
         };

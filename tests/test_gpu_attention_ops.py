@@ -289,6 +289,83 @@ def test_paged_max_q(eng):
         p.verify(max_q=m)
 
 
+def test_paged_rows_beyond_max_q_in_windows(eng):
+    """Far more rows than max_q: only the positions of the computed rows count
+    (their windows lie far before the request's end), and the call after it, which
+    splits its request, is not touched by it."""
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    a = Paged(gen, [1000, 900], [1000, 5000], 8, 2, 64, BF16, BF16, 16)
+    b = Paged(gen, [1, 1], [9000, 700], 8, 2, 64, BF16, BF16, 16)
+    for window, m in ((1, 1), (100, 2), (0, 2)):
+        a.out.fill_(7.0)
+        a.run(eng, max_q=m, window=window)
+        a.verify(window, max_q=m)
+        b.run(eng)
+        b.verify()
+
+
+@pytest.mark.parametrize("act,cache", [(F32, F16), (BF16, BF16)])
+def test_paged_widest_window(eng, act, cache):
+    """A window of 2^31 - 1 is none, also beside rows before position 0."""
+    gen = torch.Generator(device="cuda").manual_seed(16)
+    for q_lens, kv_lens in (([3, 2], [2, 300]), ([50, 40], [20, 300])):
+        p = Paged(gen, q_lens, kv_lens, 8, 2, 64, act, cache, 16)
+        p.run(eng, window=2 ** 31 - 1)
+        p.verify()
+
+
+# fp32 in workgroups of eight waves: columns for all of the device, whole heads
+@pytest.mark.parametrize("H,KVH,hd,lens,window", [(64, 8, 64, [2100], 0), (32, 8, 128, [1100, 1050], 0),
+                                                  (16, 16, 64, [4133], 0), (64, 8, 64, [2200], 300)])
+def test_packed_fp32_full_device(eng, H, KVH, hd, lens, window):
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    p = Packed(gen, lens, H, KVH, hd, F32, first=1, behind=9)
+    sk = randn(gen, (H,), F32, 2.0)
+    p.run(eng, window=window, sinks=sk)
+    p.verify(window, sk)
+
+
+@pytest.mark.parametrize("H,KVH,hd,window", [(64, 8, 64, 0), (32, 8, 128, 0), (32, 8, 128, 700)])
+@pytest.mark.parametrize("cache", [F32, F16, BF16])
+def test_paged_fp32_full_device(eng, cache, H, KVH, hd, window):
+    """A chunk of 300 rows: eight waves, keys split; pages that are none."""
+    gen = torch.Generator(device="cuda").manual_seed(18)
+    p = Paged(gen, [300], [9000], H, KVH, hd, F32, cache, 16, behind=5)
+    for b in (0, 77, 540):
+        p.tab[0][b] = -1
+    p.run(eng, window=window, max_kv=9000)
+    p.verify(window)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("q,kv", [(300, 9000), (600, 600)])
+def test_paged_specials_in_split_keys(eng, act, cache, q, kv):
+    """Values that are not finite near the causal edge and deep in the history
+    of a chunk whose keys are split: rows that see them have them, the others
+    are exact."""
+    gen = torch.Generator(device="cuda").manual_seed(19)
+    p = Paged(gen, [q], [kv], 16, 8, 64, act, cache, 32)
+    p.v[0][kv - 1, 0, 3] = float("nan")
+    p.v[0][kv - q // 2, 1, 4] = float("inf")
+    p.v[0][kv - q + 1, 2, 40] = -float("inf")
+    p.v[0][100, 3, 63] = float("inf")
+    p.k[0][kv - 7, 4, 0] = float("nan")
+    p.fill()
+    p.run(eng, max_kv=kv)
+    p.verify()
+
+
+@pytest.mark.parametrize("hd,KVH", [(64, 8), (128, 8)])
+def test_packed_fp32_specials_full_device(eng, hd, KVH):
+    gen = torch.Generator(device="cuda").manual_seed(20)
+    p = Packed(gen, [2100], 8 * KVH if hd == 64 else 4 * KVH, KVH, hd, F32)
+    p.v[2099, 1, 5] = float("nan")
+    p.v[1500, 3, 6] = float("inf")
+    p.v[3, 4, 7] = -float("inf")
+    p.run(eng)
+    p.verify()
+
+
 def test_paged_far_offsets(eng):
     """Pages whose elements lie beyond 2^31 and 2^32 elements (and 2^32 bytes)."""
     import picchio_amd as pa
