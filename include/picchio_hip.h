@@ -441,7 +441,10 @@ int pk_sampler_state(pk_engine *e, uint64_t *rng, int32_t *history_host, int cap
  * prompts that need no cache. The calls take device pointers and plain
  * numbers only, synchronise nothing and can be captured; what depends on the
  * requests' lengths is read on the device, so that a captured step serves
- * later lengths too. */
+ * later lengths too. The attention calls hand partial results through a
+ * workspace of the engine, which grows (waiting for the stream) in the first
+ * call that needs more; while capturing, such a call is refused: make one like
+ * it before. */
 
 /* Element types of activations and caches. */
 #define PK_T_F32  0
@@ -498,7 +501,7 @@ int pk_plan_pages(pk_engine *e, const pk_page_plan *p);
  * written. The slots of the rows that are not left out differ from each other.
  * Row t of q, k, v and q_out starts t * stride elements behind the pointer, its
  * heads side by side; pointers 16-byte aligned, strides multiples of 8. q_out
- * may be q; the other buffers may not overlap. The activations are of type
+ * may be q (with q's stride); the other buffers may not overlap. The activations are of type
  * `type`, and the pages of the same type or, with PK_T_F32, of any. n_heads 0:
  * no queries (q_dev and q_out_dev are not read). */
 typedef struct pk_kv_rows {
@@ -528,9 +531,15 @@ const float *pk_engine_rope(pk_engine *e, int *n_pos);
  * are fp32; with 16-bit types the probabilities are rounded to that type for the
  * product with V, with PK_T_F32 products are exact to about 2^-23. Row t of q,
  * k, v and out starts t * stride elements behind the pointer, its heads side by
- * side; pointers 16-byte aligned, strides multiples of 8, head_dim a multiple
- * of 16 up to 128; out may not overlap the inputs. max_len: a bound on the
- * prompts' lengths; rows beyond it are not computed. */
+ * side; pointers 16-byte aligned, strides multiples of 8 up to 2^26, head_dim a
+ * multiple of 16 up to 128; out may not overlap the inputs. max_len: a bound on
+ * the prompts' lengths; rows beyond it are not computed. n_heads up to 1024,
+ * n_seq up to 2^17 (every workgroup looks its prompt up among all of them),
+ * n_tokens times the heads of a group up to 2^30. Infinities and NaN: of values
+ * (V) they reach the rows that see them with a weight, as in the formula, and
+ * no other; an infinity among the queries or keys makes the rows that it is part
+ * of NaN where the formula's limit may be finite. Sums of weighted values have
+ * to stay within fp32 before they are divided by the denominator. */
 typedef struct pk_attn_packed {
     int32_t type, n_heads, n_kv_heads, head_dim;
     int32_t n_tokens, n_seq, max_len, window;
@@ -551,8 +560,8 @@ int pk_attention_packed(pk_engine *e, const pk_attn_packed *a);
  * positions up to its own, with window > 0 the last `window` of them. A position
  * on a table entry outside 0 .. n_pages - 1 is not seen; a row that sees
  * nothing is 0 (lse: its sink, or -infinity). kv_len is cut to 0 .. max_blocks *
- * page_size. max_q: a bound on a request's rows (rows beyond it are not
- * computed); max_kv: the host's bound on the lengths, which only chooses the
+ * page_size, at most 2^30. max_q: a bound on a request's rows (rows beyond it are
+ * not computed); max_kv: the host's bound on the lengths, which only chooses the
  * launch (0: max_blocks * page_size). The pages have the queries' type or, with
  * PK_T_F32, any. The rest as in pk_attention_packed. */
 typedef struct pk_attn_paged {

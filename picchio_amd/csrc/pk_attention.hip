@@ -7,6 +7,8 @@
 
 namespace {
 
+constexpr int MAX_REQ = 1 << 17;                             // (every workgroup looks through all of them)
+
 int check_common(const pk_engine *e, int H, int KVH, int hd, int n_tokens, int n_req, int max_q, int window, float scale) {
     PK_CHECK(n_tokens >= 0 && n_req >= 0 && max_q >= 0 && window >= 0, PK_ERR_ARG,
              "attention: %d rows, %d requests of up to %d rows, window %d", n_tokens, n_req, max_q, window);
@@ -15,6 +17,9 @@ int check_common(const pk_engine *e, int H, int KVH, int hd, int n_tokens, int n
     PK_CHECK(hd >= 16 && hd <= 128 && hd % 16 == 0, PK_ERR_UNSUPPORTED,
              "head_dim %d (supported: multiples of 16 up to 128)", hd);
     PK_CHECK(scale >= 0.0f && scale <= 3.4e38f, PK_ERR_ARG, "attention: scale %g", (double)scale);
+    PK_CHECK(n_req <= MAX_REQ, PK_ERR_UNSUPPORTED, "attention: %d requests (supported: up to %d)", n_req, MAX_REQ);
+    // (the kernels count columns, and positions before the first, in 32 bits)
+    PK_CHECK((int64_t)n_tokens * (H / KVH) <= 1 << 30, PK_ERR_UNSUPPORTED, "attention: %d rows of %d heads per key head", n_tokens, H / KVH);
     return PK_OK;
 }
 
@@ -52,7 +57,8 @@ extern "C" int pk_attention_packed(pk_engine *e, const pk_attn_packed *p) {
     a.q = p->q_dev, a.k = p->k_dev, a.v = p->v_dev, a.out = p->out_dev;
     a.q_stride = p->q_stride, a.k_stride = p->k_stride, a.v_stride = p->v_stride, a.out_stride = p->out_stride;
     a.cu = p->cu_dev, a.sinks = p->sinks_dev, a.lse = p->lse_dev;
-    a.n_tokens = p->n_tokens, a.n_req = p->n_seq, a.max_q = p->max_len, a.window = p->window;
+    a.n_tokens = p->n_tokens, a.n_req = p->n_seq, a.max_q = p->max_len;
+    a.window = p->window < p->n_tokens ? p->window : 0;
     a.H = p->n_heads, a.KVH = p->n_kv_heads, a.hd = p->head_dim;
     a.scale2 = (p->scale > 0.0f ? p->scale : 1.0f / sqrtf((float)p->head_dim)) * PK_LOG2E;
     a.type = a.cache_type = p->type;
@@ -66,7 +72,7 @@ extern "C" int pk_attention_paged(pk_engine *e, const pk_attn_paged *p) {
     PK_TRY(pk_check_pages(p->pages, p->type));
     const pk_pages &g = p->pages;
     PK_TRY(check_common(e, p->n_heads, g.n_kv_heads, g.head_dim, p->n_tokens, p->n_req, p->max_q, p->window, p->scale));
-    PK_CHECK(p->max_kv >= 0 && p->max_blocks > 0 && (int64_t)p->max_blocks * g.page_size <= INT32_MAX, PK_ERR_ARG,
+    PK_CHECK(p->max_kv >= 0 && p->max_blocks > 0 && (int64_t)p->max_blocks * g.page_size <= 1 << 30, PK_ERR_ARG,
              "attention_paged: tables of %d pages of %d, max_kv %d", p->max_blocks, g.page_size, p->max_kv);
     if (p->n_tokens == 0 || p->n_req == 0 || p->max_q == 0) return PK_OK;
     PK_CHECK(p->cu_q_dev && p->kv_len_dev && p->table_dev, PK_ERR_ARG, "attention_paged: null argument");
@@ -76,7 +82,7 @@ extern "C" int pk_attention_paged(pk_engine *e, const pk_attn_paged *p) {
     a.q = p->q_dev, a.k = g.k_dev, a.v = g.v_dev, a.out = p->out_dev;
     a.q_stride = p->q_stride, a.out_stride = p->out_stride;
     a.cu = p->cu_q_dev, a.kv_len = p->kv_len_dev, a.table = p->table_dev, a.sinks = p->sinks_dev, a.lse = p->lse_dev;
-    a.n_tokens = p->n_tokens, a.n_req = p->n_req, a.max_q = p->max_q, a.window = p->window;
+    a.n_tokens = p->n_tokens, a.n_req = p->n_req, a.max_q = p->max_q;
     a.H = p->n_heads, a.KVH = g.n_kv_heads, a.hd = g.head_dim;
     a.n_pages = g.n_pages, a.page_shift = __builtin_ctz((unsigned)g.page_size), a.max_blocks = p->max_blocks;
     a.scale2 = (p->scale > 0.0f ? p->scale : 1.0f / sqrtf((float)g.head_dim)) * PK_LOG2E;
@@ -84,6 +90,7 @@ extern "C" int pk_attention_paged(pk_engine *e, const pk_attn_paged *p) {
     pk_device_scope dev(e->device);
     PK_TRY(dev.rc);
     const int64_t cap = (int64_t)p->max_blocks * g.page_size;
+    a.window = p->window < cap ? p->window : 0;
     const int max_kv = (int)(p->max_kv > 0 ? std::min<int64_t>(p->max_kv, cap) : cap);
     // Few rows of every request: k_attn_few, bound by the reads of K and V. Else the
     // requests with few rows there (a tile of 128 or 256 columns would be

@@ -37,8 +37,9 @@ int pk_check_pages(const pk_pages &p, int act_type) {
 int pk_check_rows(const void *p, int64_t stride, int heads, int hd, const char *what) {
     PK_CHECK(p, PK_ERR_ARG, "%s is null", what);
     PK_CHECK(((uintptr_t)p & 15) == 0, PK_ERR_ARG, "%s: pointer not 16-byte aligned", what);
-    PK_CHECK(stride % 8 == 0 && stride >= (int64_t)heads * hd, PK_ERR_ARG,
-             "%s: row stride %lld (a multiple of 8, at least %d heads of %d)", what, (long long)stride, heads, hd);
+    // (kernels take offsets of up to eight rows in 32 bits)
+    PK_CHECK(stride % 8 == 0 && stride >= (int64_t)heads * hd && stride <= 1 << 26, PK_ERR_ARG,
+             "%s: row stride %lld (a multiple of 8, at least %d heads of %d, at most 2^26)", what, (long long)stride, heads, hd);
     return PK_OK;
 }
 

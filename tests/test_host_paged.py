@@ -116,6 +116,20 @@ for kw in both + (dict(n_seq=-1), dict(max_len=-1), dict(n_kv_heads=0), dict(n_k
     refuses(f_packed, packed(**kw), -1)
 for kw in both + (dict(n_req=-1), dict(max_q=-1), dict(max_kv=-1), dict(max_blocks=0), dict(max_blocks=1 << 28)):
     refuses(f_paged, paged(**kw), -1)
+big = 1 << 26
+for kw in (dict(q_stride=big + 8), dict(out_stride=big + 8), dict(k_stride=big + 8), dict(v_stride=1 << 40)):
+    refuses(f_packed, packed(**kw), -1)
+takes(f_packed, packed(q_stride=big, k_stride=big, v_stride=big, out_stride=big))
+refuses(f_paged, paged(q_stride=big + 8), -1)
+refuses(f_rows, rows(v_stride=big + 8), -1)
+refuses(f_paged, paged(max_blocks=(1 << 26) + 1), -1)             # 2^30 positions of 16
+refuses(f_packed, packed(n_seq=(1 << 17) + 1), -4)
+refuses(f_paged, paged(n_req=(1 << 17) + 1), -4)
+takes(f_paged, paged(n_req=1 << 17))
+refuses(f_packed, packed(n_tokens=(1 << 29) + 1), -4)             # two heads to a key head
+refuses(f_paged, paged(n_tokens=(1 << 29) + 1), -4)
+for f, make in ((f_packed, packed), (f_paged, paged)):
+    takes(f, make(window=2 ** 31 - 1))
 for hd in (8, 24, 100, 144, 256):
     refuses(f_packed, packed(head_dim=hd), -4)
 refuses(f_packed, packed(n_heads=1026, q_stride=1 << 17, out_stride=1 << 17), -4)
