@@ -632,7 +632,10 @@ int launch(pk_engine *e, const pk_attn_args &a, int64_t tiles) {
     // and never more than the tiles; the split requests' parts at most 2 W, since each of them is
     // longer than a chunk
     const int64_t slots = (FEW_PER_CU * (int64_t)e->n_cu + a.KVH - 1) / a.KVH;
-    const int W = (int)std::max<int64_t>(slots, 1);
+    // (Requests up to twice as many: two rounds of half as long chunks. 48 requests of up to 4000
+    // positions, 16 KV heads of 128, 134 us, 177 with one round's chunks; 70 of up to 8000, 8 of 64,
+    // 88 / 94; but 200 of up to 2000 92 / 89.)
+    const int W = (int)std::max<int64_t>(slots, 1) * (a.n_req > slots && a.n_req <= 2 * slots ? 2 : 1);
     const int64_t grid = std::min<int64_t>(W + (int64_t)a.n_req, std::max<int64_t>(tiles, 1));
     PK_TRY(pk_attn_workspace(e, (int64_t)a.KVH * 2 * W * 16 * NQ * (HDP + 2), (int64_t)a.KVH * 2 * W));
     k_attn_few<A, C, HDP, NQ><<<dim3((unsigned)grid, (unsigned)a.KVH), FEW_THREADS, 0, e->stream>>>(a, W, 2 * W, e->att_ws, e->att_cnt);

@@ -594,39 +594,57 @@ __global__ __launch_bounds__(64 * WV, tile_simd(HDP, QP)) void k_attn_tile(pk_at
     }
 }
 
-// The parts of split keys, added up in order: four elements of a column per thread.
-constexpr int JOIN_THREADS = 256;
+// The parts of split keys, added up in order: four elements of a column per thread, the
+// loads of JOIN_AHEAD parts in flight (one after the other: 64 rows after 100,000
+// positions, 32 parts, 50 us for 15). Bound by latency, or by the reads of many columns.
+constexpr int JOIN_THREADS = 256, JOIN_AHEAD = 8;
 template <typename A, int BM, int HDP, int KT>
 __global__ __launch_bounds__(JOIN_THREADS) void k_attn_join(pk_attn_args a, int cut, int splits, const float *__restrict__ part) {
     __shared__ int found;
-    const int kvh = blockIdx.x % a.KVH, G = a.H / a.KVH, quads = a.hd >> 2;
+    const int kvh = blockIdx.x % a.KVH, G = a.H / a.KVH;
     const int64_t slot = blockIdx.x / a.KVH;
     const place pl = find<BM, KT>(a, slot, cut, &found);
     if (pl.r < 0) return;
-    const float *src = part + (slot * a.KVH + kvh) * splits * (BM * (HDP + 2));
-    const int cols = min(BM, pl.n_idx - pl.idx0);
-    for (int x = blockIdx.y * JOIN_THREADS + threadIdx.x; x < cols * quads; x += gridDim.y * JOIN_THREADS) {
-        const int col = x / quads, e = (x - col * quads) * 4, idx = pl.idx0 + col, i = idx / G, hq = kvh * G + (idx - i * G);
-        const float sk = a.sinks ? a.sinks[hq] * PK_LOG2E : -INFINITY;
-        float top = sk;
-        for (int y = 0; y < splits; ++y) top = fmaxf(top, src[(int64_t)y * (BM * (HDP + 2)) + col]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        float l = __builtin_amdgcn_exp2f(sk - ref);
-        f32x4 acc = {0, 0, 0, 0};
-        for (int y = 0; y < splits; ++y) {
-            const float *p = src + (int64_t)y * (BM * (HDP + 2));
-            if (pl.n_t * (int64_t)y / splits == pl.n_t * (int64_t)(y + 1) / splits) continue;     // no keys
-            const float f = __builtin_amdgcn_exp2f(p[col] - ref);
-            l = __builtin_fmaf(p[BM + col], f, l);
-            const f32x4 v = *reinterpret_cast<const f32x4 *>(p + 2 * BM + (int64_t)col * HDP + e);
+    constexpr int PART = BM * (HDP + 2), QUADS = HDP / 4;
+    const int x = blockIdx.y * JOIN_THREADS + threadIdx.x, col = x / QUADS, e = x % QUADS * 4, idx = pl.idx0 + col;
+    if (idx >= pl.n_idx || e >= a.hd) return;
+    const float *src = part + (slot * a.KVH + kvh) * splits * PART;
+    const int i = idx / G, hq = kvh * G + (idx - i * G);
+    const float sk = a.sinks ? a.sinks[hq] * PK_LOG2E : -INFINITY;
+    float top = sk, l = sk > -INFINITY ? 1.0f : 0.0f;
+    f32x4 acc = {0, 0, 0, 0};
+    for (int y0 = 0; y0 < splits; y0 += JOIN_AHEAD) {
+        float m[JOIN_AHEAD], s[JOIN_AHEAD];
+        f32x4 v[JOIN_AHEAD];
 #pragma unroll
-            for (int z = 0; z < 4; ++z) acc[z] = __builtin_fmaf(v[z], f, acc[z]);
+        for (int y = 0; y < JOIN_AHEAD; ++y) {
+            m[y] = -INFINITY;
+            if (y0 + y >= splits) continue;
+            const float *p = src + (int64_t)(y0 + y) * PART;
+            m[y] = p[col], s[y] = p[BM + col];
+            v[y] = *reinterpret_cast<const f32x4 *>(p + 2 * BM + (int64_t)col * HDP + e);
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const int64_t row = pl.s.row0 + i;
-        store4((A *)a.out + row * a.out_stride + (int64_t)hq * a.hd + e, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
-        if (a.lse && e == 0) a.lse[row * a.H + hq] = l == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * PK_LN2;
+        float mn = top;
+#pragma unroll
+        for (int y = 0; y < JOIN_AHEAD; ++y) mn = fmaxf(mn, m[y]);
+        const float ref = mn == -INFINITY ? 0.0f : mn, f0 = __builtin_amdgcn_exp2f(top - ref);
+        top = mn;
+        l *= f0;
+        acc *= f0;
+#pragma unroll
+        for (int y = 0; y < JOIN_AHEAD; ++y) {
+            // (parts without keys hold no sums)
+            if (y0 + y >= splits || pl.n_t * (int64_t)(y0 + y) / splits == pl.n_t * (int64_t)(y0 + y + 1) / splits) continue;
+            const float f = __builtin_amdgcn_exp2f(m[y] - ref);
+            l = __builtin_fmaf(s[y], f, l);
+#pragma unroll
+            for (int z = 0; z < 4; ++z) acc[z] = __builtin_fmaf(v[y][z], f, acc[z]);
+        }
     }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int64_t row = pl.s.row0 + i;
+    store4((A *)a.out + row * a.out_stride + (int64_t)hq * a.hd + e, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    if (a.lse && e == 0) a.lse[row * a.H + hq] = l == 0.0f ? -INFINITY : ((top == -INFINITY ? 0.0f : top) + __builtin_amdgcn_logf(l)) * PK_LN2;
 }
 
 template <typename T, typename A, typename C, int HDP, int WV, int QP, int KP, bool PAGED, bool FULL>
@@ -649,7 +667,7 @@ int launch(pk_engine *e, const pk_attn_args &a, int cut, int max_kv) {
         <<<dim3((unsigned)wgs, (unsigned)splits), 64 * WV, 0, e->stream>>>(a, cut, splits, part);
     PK_HIP(hipGetLastError());
     if (splits > 1) {
-        k_attn_join<A, BM, HDP, KT><<<dim3((unsigned)wgs, BM / 32), JOIN_THREADS, 0, e->stream>>>(a, cut, splits, part);
+        k_attn_join<A, BM, HDP, KT><<<dim3((unsigned)wgs, BM * HDP / 4 / JOIN_THREADS), JOIN_THREADS, 0, e->stream>>>(a, cut, splits, part);
         PK_HIP(hipGetLastError());
     }
     return PK_OK;
