@@ -17,6 +17,12 @@
 // order. (Equal shares of one line of tiles instead, across requests, left a
 // workgroup with the parts of several, one after the other: 32 requests with
 // 128-position windows 23 us, as items 12.)
+//
+// Measured, 64 query heads over 8 of 64, the bytes of K and V per second: 32 requests of
+// up to 8192 positions, bf16, 51 us, 3.75 TB/s; one of 100,001, fp32 over fp16, 51 us,
+// 4.0 TB/s; 32 of 128-element heads 72 us, 4.3 TB/s; what is missing to a copy's 5.2 is the
+// start (a workgroup's request, its pages, the first keys: four loads that wait for
+// each other) and the join.
 #include "pk_attention.h"
 
 namespace {
@@ -116,32 +122,24 @@ __device__ __forceinline__ int wave_scan(int v) {
     return dpp_add<0x143, 0xc>(v);
 }
 
-template <typename A, typename C, int HDP, int NQ>
-__global__ __launch_bounds__(FEW_THREADS, FEW_PER_CU) void k_attn_few(pk_attn_args a, int W, int max_parts, float *part, uint32_t *count) {
-    constexpr bool F32 = sizeof(C) == 4;                        // fp32 cache: fp32 products
-    // fp32 queries and probabilities over a 16-bit cache: as planes of the cache's type, whose
-    // products are exact. bf16: three, 8 bits each. fp16: two, 11 bits each, of values
-    // scaled to at most 2^14, so that the low plane's last bit is at 2^-38 of that.
-    constexpr int QP = F32 || sizeof(A) == 2 ? 1 : __is_same(C, pk_f16) ? 2 : 3;
-    constexpr float SHIFT = __is_same(C, pk_f16) ? 14.0f : 0.0f;    // probabilities are at most 2^SHIFT
-    typedef typename regs<C, 8>::type c8;
-    constexpr int KT = few_tile(HDP * (int)sizeof(C), NQ), NB = KT / 16;
-    constexpr int KE = HDP / 4, KV8 = KE / 8;                   // elements of a key per lane, in vectors of 8
-    constexpr int VE = HDP / 16;                                // elements of a value per lane
-    constexpr int COLS = 16 * NQ, LD = HDP + 4;
-    typedef typename regs<C, 8>::type k8;
-    typedef typename regs<C, VE>::type vrow;
-
-    __shared__ __attribute__((aligned(16))) float so[FEW_WAVES][COLS][LD];
-    __shared__ float sm[FEW_WAVES][COLS], sl[FEW_WAVES][COLS];
-    __shared__ double wave_tiles[FEW_WAVES];
-    __shared__ int wave_items[FEW_WAVES][2], found[4], last_in;
-
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m16 = lane & 15;
-    const int kvh = blockIdx.y, G = a.H / a.KVH, hd = a.hd;
-    const int ps = 1 << a.page_shift;
-
-    // ── this workgroup's item ──
+// A workgroup's item: request r (< 0: none), part `it` of n_it, the first of them part0 among the
+// parts of split requests.
+struct piece {
+    int r, it, n_it, part0;
+};
+struct find_lds {
+    double tiles[FEW_WAVES];
+    int items[FEW_WAVES][2], found[4];
+};
+template <int KT>
+__device__ __forceinline__ piece few_find(const pk_attn_args &a, int W, find_lds &lds) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // equal chunks of the one request: nothing to search (37 positions 8.7 us with the
+    // search, 7.6 without)
+    if (a.n_req == 1) {
+        const int t = few_seg<KT>(a, 0).tiles, chunk = max((t + W - 1) / W, FEW_WAVES), n = (t + chunk - 1) / chunk;
+        return {(int)blockIdx.x < n ? 0 : -1, (int)blockIdx.x, max(n, 1), 0};
+    }
     // Up to 64 FEW_KEPT requests: each wave finds it for itself, a lane for every 64th of the
     // requests, with no barriers (~1 us). More: a thread for every 256th.
     const bool wide = a.n_req > 64 * FEW_KEPT;
@@ -161,9 +159,9 @@ __global__ __launch_bounds__(FEW_THREADS, FEW_PER_CU) void k_attn_few(pk_attn_ar
     each([&](int, int n) { all += n; return false; });
     all = pk_wave_sum_d(all);                                   // (exact)
     if (wide) {
-        if (lane == 0) wave_tiles[wave] = all;
+        if (lane == 0) lds.tiles[wave] = all;
         __syncthreads();
-        all = wave_tiles[0] + wave_tiles[1] + wave_tiles[2] + wave_tiles[3];
+        all = lds.tiles[0] + lds.tiles[1] + lds.tiles[2] + lds.tiles[3];
     }
     // The shortest chunk, from an equal share of the tiles for each of W workgroups on, with which
     // the items are at most W (give or take one for the division): all run at once, the
@@ -193,10 +191,10 @@ __global__ __launch_bounds__(FEW_THREADS, FEW_PER_CU) void k_attn_few(pk_attn_ar
     });
     int at = wave_scan(items), part_at = wave_scan(parts);
     if (wide) {
-        if (lane == 63) wave_items[wave][0] = at, wave_items[wave][1] = part_at;
-        if (tid == 0) found[0] = -1;
+        if (lane == 63) lds.items[wave][0] = at, lds.items[wave][1] = part_at;
+        if (tid == 0) lds.found[0] = -1;
         __syncthreads();
-        for (int i = 0; i < wave; ++i) at += wave_items[i][0], part_at += wave_items[i][1];
+        for (int i = 0; i < wave; ++i) at += lds.items[i][0], part_at += lds.items[i][1];
     }
     at -= items;
     part_at -= parts;
@@ -215,11 +213,40 @@ __global__ __launch_bounds__(FEW_THREADS, FEW_PER_CU) void k_attn_few(pk_attn_ar
     int r = whose ? __builtin_amdgcn_readlane(my_r, src) : -1, n_it = __builtin_amdgcn_readlane(my_n, src);
     int it = (int)blockIdx.x - __builtin_amdgcn_readlane(at, src), part0 = __builtin_amdgcn_readlane(part_at, src);
     if (wide) {
-        if (whose && lane == 0) found[0] = r, found[1] = n_it, found[2] = it, found[3] = part0;
+        if (whose && lane == 0) lds.found[0] = r, lds.found[1] = n_it, lds.found[2] = it, lds.found[3] = part0;
         __syncthreads();
-        r = __builtin_amdgcn_readfirstlane(found[0]), n_it = __builtin_amdgcn_readfirstlane(found[1]);
-        it = __builtin_amdgcn_readfirstlane(found[2]), part0 = __builtin_amdgcn_readfirstlane(found[3]);
+        r = __builtin_amdgcn_readfirstlane(lds.found[0]), n_it = __builtin_amdgcn_readfirstlane(lds.found[1]);
+        it = __builtin_amdgcn_readfirstlane(lds.found[2]), part0 = __builtin_amdgcn_readfirstlane(lds.found[3]);
     }
+    return {r, it, n_it, part0};
+}
+
+template <typename A, typename C, int HDP, int NQ>
+__global__ __launch_bounds__(FEW_THREADS, FEW_PER_CU) void k_attn_few(pk_attn_args a, int W, int max_parts, float *part, uint32_t *count) {
+    constexpr bool F32 = sizeof(C) == 4;                        // fp32 cache: fp32 products
+    // fp32 queries and probabilities over a 16-bit cache: as planes of the cache's type, whose
+    // products are exact. bf16: three, 8 bits each. fp16: two, 11 bits each, of values
+    // scaled to at most 2^14, so that the low plane's last bit is at 2^-38 of that.
+    constexpr int QP = F32 || sizeof(A) == 2 ? 1 : __is_same(C, pk_f16) ? 2 : 3;
+    constexpr float SHIFT = __is_same(C, pk_f16) ? 14.0f : 0.0f;    // probabilities are at most 2^SHIFT
+    typedef typename regs<C, 8>::type c8;
+    constexpr int KT = few_tile(HDP * (int)sizeof(C), NQ), NB = KT / 16;
+    constexpr int KE = HDP / 4, KV8 = KE / 8;                   // elements of a key per lane, in vectors of 8
+    constexpr int VE = HDP / 16;                                // elements of a value per lane
+    constexpr int COLS = 16 * NQ, LD = HDP + 4;
+    typedef typename regs<C, 8>::type k8;
+    typedef typename regs<C, VE>::type vrow;
+
+    __shared__ __attribute__((aligned(16))) float so[FEW_WAVES][COLS][LD];
+    __shared__ float sm[FEW_WAVES][COLS], sl[FEW_WAVES][COLS];
+    __shared__ find_lds lds;
+    __shared__ int last_in;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m16 = lane & 15;
+    const int kvh = blockIdx.y, G = a.H / a.KVH, hd = a.hd;
+    const int ps = 1 << a.page_shift;
+
+    const auto [r, it, n_it, part0] = few_find<KT>(a, W, lds);
     if (r < 0) return;
     const seg sg = few_seg<KT>(a, r);
     const int t0 = (int)((int64_t)sg.tiles * it / n_it), t1 = (int)((int64_t)sg.tiles * (it + 1) / n_it);

