@@ -46,13 +46,13 @@ int pk_check_rows(const void *p, int64_t stride, int heads, int hd, const char *
 namespace {
 
 // ───────────────────────── pages of a step ─────────────────────────
-// One launch: bound by its latency (a step of 32 requests 6.7 us) and, for long
+// One launch: bound by its latency (a step of 32 requests 6.3 us) and, for long
 // prompts, by the write of the rows. Every workgroup adds up the requests' pages
 // and rows for itself (three running sums over at most 4096 requests, ~1 us) and
 // keeps row starts, page places and old lengths in LDS; then it moves the pages of
 // its share of the requests and writes its share of the rows, four neighbours per
 // thread, which find their request once and write 16 bytes (1000 requests, 1.3 M
-// rows: 12.6 us, one row per thread 15.3). Two launches, sums first, would save the
+// rows: 11.4 us, one row per thread 15.3). Two launches, sums first, would save the
 // repeated sums but cost a launch more than those. What a workgroup reads of the
 // table and the ring (pages below ceil(old / page_size); the ring's free entries)
 // no other one writes; the ring's state is written by the workgroup that arrives
@@ -171,16 +171,18 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_plan_pages(
         for (int r = last + 1 + t; r <= n_req; r += PLAN_THREADS) cu[r] = cu[last];
         __syncthreads();
     }
-    // The state is read; the last workgroup to have done so writes it. Arrivals in two
-    // steps, 16 words and then one (650 on one word take 10 us), by a wave while the others go on.
+    // The state is read; the last workgroup to have done so writes it, by a wave while the others
+    // go on. Many arrive in two steps, at 16 words and then one (650 on one word take 10 us).
     if (t == PLAN_THREADS - 64) {
         const auto arrive = [&](uint32_t *c, uint32_t of) {
+            if (of == 1) return true;
             const bool last_in = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == of;
             if (last_in) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             return last_in;
         };
-        const uint32_t group = blockIdx.x & 15, groups = min(gridDim.x, 16u);
-        if (arrive(arrivals + 16 * (1 + group), (gridDim.x + 15 - group) >> 4) && arrive(arrivals, groups)) {
+        const uint32_t group = blockIdx.x & 15;
+        if (gridDim.x <= 32 ? arrive(arrivals, gridDim.x)
+                            : arrive(arrivals + 16 * (1 + group), (gridDim.x + 15 - group) >> 4) && arrive(arrivals, 16)) {
             state[0] = (int32_t)(((uint32_t)head + (uint32_t)moved[0]) % (uint32_t)n_pages);
             state[1] = min(count - moved[0] + moved[1], n_pages);
         }
@@ -228,28 +230,29 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_plan_pages(
     for (int64_t base = (int64_t)blockIdx.x * PLAN_ROWS; base < max_tokens; base += (int64_t)gridDim.x * PLAN_ROWS) {
         const int64_t i0 = base + t * 4;
         int p[4], s[4];
-        int r = -1, end = 0, off = 0, ob = 0, k_at = -1, page = -1;
+        const int32_t *src[4];                                  // the entry that names the row's page
+        int r = -1, end = 0, off = 0, ob = 0;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int64_t i = i0 + q;
-            p[q] = 0, s[q] = -1;
+            p[q] = 0;
+            src[q] = nullptr;
             if (i >= total) continue;
-            if (r < 0 || i >= end) {
-                r = find((int)i, r + 1, n_req - 1);
+            if (r < 0 || i >= end) {                            // (often the next request's)
+                r = r >= 0 && cu[r + 2] > i ? r + 1 : find((int)i, r + 1, n_req - 1);
                 end = cu[r + 1];
                 const int o = old[r];
                 off = o - cu[r];
                 ob = (o + up) >> shift;
-                k_at = -1;
             }
             p[q] = off + (int)i;
             const int k = p[q] >> shift;
-            if (k != k_at) {
-                k_at = k;
-                page = k < ob ? table[(int64_t)r * max_blocks + k] : ring[from(place[r], k - ob)];
-            }
-            if (page >= 0 && page < n_pages) s[q] = (page << shift) + (p[q] & up);
+            src[q] = k < ob ? table + (int64_t)r * max_blocks + k : ring + from(place[r], k - ob);
         }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s[q] = src[q] ? *src[q] : -1;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s[q] = s[q] >= 0 && s[q] < n_pages ? (s[q] << shift) + (p[q] & up) : -1;
         if (wide && i0 + 3 < max_tokens) {
             *reinterpret_cast<int4 *>(slot + i0) = int4{s[0], s[1], s[2], s[3]};
             *reinterpret_cast<int4 *>(pos + i0) = int4{p[0], p[1], p[2], p[3]};
