@@ -452,7 +452,35 @@ def test_same_bits_again(eng, dtype):
         assert all(torch.equal(x, y) for x, y in zip(s, seen[0]))
 
 
-@pytest.mark.parametrize("n", [64, 65, 200, 256, 257, 1000])
+def test_two_engines_at_once(eng, gpu):
+    """Calls of two engines run beside each other, each on its own stream with its
+    own workspace: split decode steps, mixed steps, and a torch stream's work
+    between them."""
+    import picchio_amd as pa
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    with pa.Engine(pa.gptoss_cfg(n_layers=1, n_experts=4, ctx_len=16, vocab=64)) as other:
+        a = Paged(gen, [1, 1, 1], [9000, 20, 700], 8, 1, 64, F32, F16, 16)
+        b = Paged(gen, [60, 1, 3], [7000, 4000, 2000], 8, 1, 64, F32, F16, 16)
+        ra, rb = a.record(), b.record()
+        for e in (eng, other):                                         # sizes the workspaces
+            e.attention_paged(ra), e.attention_paged(rb)
+            e.sync()
+        a.out.fill_(7.0), b.out.fill_(7.0)
+        noise = torch.zeros(1 << 20, device="cuda")
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        for _ in range(20):
+            eng.attention_paged(ra)
+            other.attention_paged(rb)
+            with torch.cuda.stream(side):
+                noise += 1.0
+        eng.sync(), other.sync()
+        torch.cuda.synchronize()
+        a.verify(what="first"), b.verify(what="second")
+        assert (noise == 20.0).all()
+
+
+@pytest.mark.parametrize("n", [64, 65, 100, 128, 129, 200, 256, 257, 1000])
 def test_paged_many_requests(eng, n):
     """More requests than a wave's lanes or a workgroup finds at once: some idle,
     one far longer than the others, some of several rows."""

@@ -69,6 +69,26 @@ def test_plan_steps(eng, n, blocks, n_pages, page, tokens):
     random_steps(Plan(eng, n, blocks, n_pages, page, tokens, n), n, blocks * page, n + 1, 6)
 
 
+def test_plan_many_rows(eng):
+    """Rows for more workgroups than arrive on one word, captured and replayed too;
+    the rows' arrays off 16 bytes."""
+    import picchio_amd as pa
+    p = Plan(eng, 20, 300, 6100, 32, 150001, 1)
+    random_steps(p, 20, 9600, 2, 4)
+    p = Plan(eng, 20, 300, 6100, 32, 150001, 2)
+    torch.cuda.synchronize()
+    eng.capture_begin()
+    eng.plan_pages(p.call)
+    g = eng.capture_end()
+    random_steps(p, 20, 9600, 3, 4, lambda: eng.graph_launch(g))
+    eng.graph_destroy(g)
+    p = Plan(eng, 20, 300, 6100, 32, 70001, 3)
+    for name in ("slot", "pos"):
+        p.out[name] = ints([-9] * 70002)[1:]
+    p.call = pa.page_plan(p.old, p.new, p.d["table"], p.d["ring"], p.d["state"], 32, **p.out)
+    random_steps(p, 20, 9600, 4, 4)
+
+
 def test_plan_edges(eng):
     p = Plan(eng, 3, 4, 6, 16, 50)
     assert p.step([0, 0, 0], [16, 17, 1]) == [16, 17, 1]                    # a full page, one over, one row
