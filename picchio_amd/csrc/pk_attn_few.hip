@@ -226,7 +226,9 @@ __global__ __launch_bounds__(FEW_THREADS, FEW_PER_CU) void k_attn_few(pk_attn_ar
     constexpr bool F32 = sizeof(C) == 4;                        // fp32 cache: fp32 products
     // fp32 queries and probabilities over a 16-bit cache: as planes of the cache's type, whose
     // products are exact. bf16: three, 8 bits each. fp16: two, 11 bits each, of values
-    // scaled to at most 2^14, so that the low plane's last bit is at 2^-38 of that.
+    // scaled to at most 2^14, so that the low plane's last bit is at 2^-38 of that. With 16-bit
+    // queries a probability is rounded once, to the type that the product takes and the result
+    // has; the sum of them takes it unrounded.
     constexpr int QP = F32 || sizeof(A) == 2 ? 1 : __is_same(C, pk_f16) ? 2 : 3;
     constexpr float SHIFT = __is_same(C, pk_f16) ? 14.0f : 0.0f;    // probabilities are at most 2^SHIFT
     typedef typename regs<C, 8>::type c8;

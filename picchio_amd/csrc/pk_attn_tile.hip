@@ -505,7 +505,9 @@ __global__ __launch_bounds__(64 * WV, tile_simd(HDP, QP)) void k_attn_tile(pk_at
                     x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][y >> 1][8 * (y & 1) + i], scale2, -ref));
                     sum += x[i];
                 }
-                t8 pp[QP];                                      // (16-bit types: the one rounding of a probability)
+                // (16-bit types: the one rounding of a probability, half a step of the type that
+                // the product takes and that the result is rounded to as well; the sum has it unrounded)
+                t8 pp[QP];
                 planes<T, QP>(x, pp);
 #pragma unroll
                 for (int n = 0; n < QP; ++n) p[u][n][y] = pp[n];
