@@ -593,61 +593,61 @@ __global__ __launch_bounds__(FEW_THREADS, FEW_PER_CU) void k_attn_few(pk_attn_ar
                 const auto at = [&](int y) { return (const uint64_t *)(first + y * PART); };
                 const auto ld = [](const uint64_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
                 const int np = n_it;
-                // references and sums: a wave per column, a lane per part
-                for (int c = wave; c < cols; c += FEW_WAVES) {
-                    const int h = kvh * G + c % G;
-                    const float sk = a.sinks ? a.sinks[h] * PK_LOG2E : -INFINITY;
-                    float top = sk;
-                    for (int y = lane; y < np; y += 64) top = fmaxf(top, __uint_as_float((uint32_t)ld(at(y) + c)));
-                    top = pk_wave_max_f(top);
-                    const float ref = top == -INFINITY ? 0.0f : top;
-                    float l = lane == 0 ? __builtin_amdgcn_exp2f(sk - ref) : 0.0f;
-                    for (int y = lane; y < np; y += 64) {
-                        const uint64_t v = ld(at(y) + c);
-                        l = __builtin_fmaf(__uint_as_float((uint32_t)(v >> 32)), __builtin_amdgcn_exp2f(__uint_as_float((uint32_t)v) - ref), l);
-                    }
-                    l = pk_wave_sum_f(l);
-                    if (lane == 0) sm[0][c] = ref, sl[0][c] = l;
-                }
-                __syncthreads();
-                // the sums: four elements of a column per thread, the parts over as many groups of
-                // threads as there are, 8 of a group's parts in flight
+                // four elements of a column per thread, the parts over as many groups of threads as
+                // there are, 8 of a group's parts in flight: a running reference, the sum and the
+                // sums of values, in the order of the parts. (References and sums first, in
+                // a pass of their own: a round trip more, 1 us.)
                 const int items = cols * quads, groups = max(1, FEW_THREADS / items), grp = tid / items;
                 f32x4 *sums = reinterpret_cast<f32x4 *>(&so[0][0][0]);
+                float *ms = reinterpret_cast<float *>(sums + FEW_THREADS), *ls = ms + FEW_THREADS;
+                static_assert(sizeof(so) >= FEW_THREADS * 24);
+                const auto add = [](float &top, float &l, f32x4 &acc, float m, float lp, const f32x4 &v) {
+                    // (a factor of 0 stays one beside an infinity)
+                    const float mn = fmaxf(top, m), ref = mn == -INFINITY ? 0.0f : mn;
+                    const float f0 = __builtin_amdgcn_exp2f(top - ref), f1 = __builtin_amdgcn_exp2f(m - ref);
+                    top = mn;
+                    l = __builtin_fmaf(lp, f1, l * f0);
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        if (f0 != 1.0f) acc[z] = f0 == 0.0f ? 0.0f : acc[z] * f0;
+                        if (f1 != 0.0f) acc[z] = __builtin_fmaf(v[z], f1, acc[z]);
+                    }
+                };
+                const auto end = [&](int c, int e, float top, float l, f32x4 acc) {
+                    const float sk = a.sinks ? a.sinks[kvh * G + c % G] * PK_LOG2E : -INFINITY;
+                    add(top, l, acc, sk, sk > -INFINITY ? 1.0f : 0.0f, f32x4{0, 0, 0, 0});
+                    finish(sg, kvh, G, c, e, acc, l, top == -INFINITY ? 0.0f : top);
+                };
                 for (int x = groups > 1 ? tid - grp * items : tid; x < items && grp < groups; x += FEW_THREADS) {
                     const int c = x / quads, e = (x - c * quads) * 4;
-                    const float ref = sm[0][c];
+                    float top = -INFINITY, l = 0.0f;
                     f32x4 acc = {0, 0, 0, 0};
                     for (int y0 = grp; y0 < np; y0 += 8 * groups) {
-                        uint64_t m[8], v[8][2];
+                        uint64_t ml[8], v[8][2];
 #pragma unroll
                         for (int y = 0; y < 8; ++y) {
                             const uint64_t *p = at(min(y0 + y * groups, np - 1));
-                            m[y] = ld(p + c);
+                            ml[y] = ld(p + c);
                             v[y][0] = ld(p + (2 * COLS + c * HDP + e) / 2);
                             v[y][1] = ld(p + (2 * COLS + c * HDP + e) / 2 + 1);
                         }
 #pragma unroll
-                        for (int y = 0; y < 8; ++y) {
-                            const float f = y0 + y * groups < np ? __builtin_amdgcn_exp2f(__uint_as_float((uint32_t)m[y]) - ref) : 0.0f;
-                            if (f == 0.0f) continue;
-                            const float *ov = reinterpret_cast<const float *>(v[y]);
-#pragma unroll
-                            for (int z = 0; z < 4; ++z) acc[z] = __builtin_fmaf(ov[z], f, acc[z]);
-                        }
+                        for (int y = 0; y < 8; ++y)
+                            if (y0 + y * groups < np)
+                                add(top, l, acc, __uint_as_float((uint32_t)ml[y]), __uint_as_float((uint32_t)(ml[y] >> 32)),
+                                    *reinterpret_cast<const f32x4 *>(v[y]));
                     }
-                    if (groups > 1) sums[tid] = acc;
-                    else finish(sg, kvh, G, c, e, acc, sl[0][c], ref);
+                    if (groups > 1) sums[tid] = acc, ms[tid] = top, ls[tid] = l;
+                    else end(c, e, top, l, acc);
                 }
                 if (groups > 1) {
                     __syncthreads();
                     if (tid < items) {
                         f32x4 acc = sums[tid];
-                        for (int y = 1; y < groups; ++y)
-#pragma unroll
-                            for (int z = 0; z < 4; ++z) acc[z] += sums[y * items + tid][z];
+                        float top = ms[tid], l = ls[tid];
+                        for (int y = 1; y < groups; ++y) add(top, l, acc, ms[y * items + tid], ls[y * items + tid], sums[y * items + tid]);
                         const int c = tid / quads;
-                        finish(sg, kvh, G, c, (tid - c * quads) * 4, acc, sl[0][c], sm[0][c]);
+                        end(c, (tid - c * quads) * 4, top, l, acc);
                     }
                 }
             }
