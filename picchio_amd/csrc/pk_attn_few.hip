@@ -19,7 +19,7 @@
 // 128-position windows 23 us, as items 12.)
 //
 // Measured, 64 query heads over 8 of 64, the bytes of K and V per second: 32 requests of
-// up to 8192 positions, bf16, 51 us, 3.75 TB/s; one of 100,001, fp32 over fp16, 51 us,
+// up to 8192 positions, bf16, 50 us, 3.8 TB/s; one of 100,001, fp32 over fp16, 51 us,
 // 4.0 TB/s; 32 of 128-element heads 72 us, 4.3 TB/s; what is missing to a copy's 5.2 is the
 // start (a workgroup's request, its pages, the first keys: four loads that wait for
 // each other) and the join.
@@ -391,26 +391,45 @@ __global__ __launch_bounds__(FEW_THREADS, FEW_PER_CU) void k_attn_few(pk_attn_ar
             const bool masked = (ok_now & all) != all || base + KT - 1 > p_first || (a.window > 0 && base <= p_last - a.window);
             uint64_t odd = 0;                                   // keys with values that are added one by one
             if (masked) {
-                // (the empty asm keeps this a branch: as selects it would be work of every tile)
-                uint64_t mine = ok_now >> (4 * g);
-                asm volatile("" : "+v"(mine));
+                // (the empty asm keeps these branches: as selects they would be work of every tile)
+                if (base + KT - 1 > p_first)
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
+                    for (int n = 0; n < NQ; ++n) {
+                        int upto = pos[n] - base - 4 * g;
+                        asm volatile("" : "+v"(upto));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = base + b * 16 + 4 * g + i;
-                        const bool there = mine >> (b * 16 + i) & 1;
+                        for (int b = 0; b < NB; ++b)
 #pragma unroll
-                        for (int n = 0; n < NQ; ++n) {
-                            const bool see = there && j <= pos[n] && (a.window <= 0 || j > pos[n] - a.window);
-                            if (!see) s[n][b][i] = -INFINITY;
-                        }
-                        const bool none = !there || j > p_last || (a.window > 0 && j <= p_first - a.window);
-                        if (none) v[b][i] = vrow{};             // 0 x NaN
+                            for (int i = 0; i < 4; ++i)
+                                if (b * 16 + i > upto) s[n][b][i] = -INFINITY;
                     }
+                if (a.window > 0 && base <= p_last - a.window)
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        int from = pos[n] - a.window - base - 4 * g;
+                        asm volatile("" : "+v"(from));
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (b * 16 + i <= from) s[n][b][i] = -INFINITY;
+                    }
+                if ((ok_now & all) != all) {
+                    uint64_t mine = ok_now >> (4 * g);
+                    asm volatile("" : "+v"(mine));
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool there = mine >> (b * 16 + i) & 1;
+#pragma unroll
+                            for (int n = 0; n < NQ; ++n)
+                                if (!there) s[n][b][i] = -INFINITY;
+                        }
+                }
             }
             // Values that are not finite: with planes they meet zeros, and where some rows do not
-            // see them, zero probabilities.
+            // see them (or the place holds no position), zero probabilities.
             if (masked || QP > 1) {
                 uint32_t any = 0;
 #pragma unroll
@@ -423,7 +442,7 @@ __global__ __launch_bounds__(FEW_THREADS, FEW_PER_CU) void k_attn_few(pk_attn_ar
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int j = base + b * 16 + 4 * g + i;
-                            const bool every = j <= p_first && (a.window <= 0 || j > p_last - a.window);
+                            const bool every = (ok_now >> (j - base) & 1) && j <= p_first && (a.window <= 0 || j > p_last - a.window);
                             const uint64_t who = __ballot(odd_row<C, VE>(v[b][i]) != 0 && VE * m16 < hd && (QP > 1 || !every));
 #pragma unroll
                             for (int gg = 0; gg < 4; ++gg)
@@ -495,6 +514,7 @@ __global__ __launch_bounds__(FEW_THREADS, FEW_PER_CU) void k_attn_few(pk_attn_ar
             while (odd) {
                 const int jj = __ffsll((unsigned long long)odd) - 1, j = base + jj;
                 odd &= odd - 1;
+                if (!(ok_now >> jj & 1)) continue;
                 const int pg = tab[j >> a.page_shift];          // (a page: `there`)
                 const C *src = (const C *)a.v + row_at(pg, j);
 #pragma unroll
