@@ -30,7 +30,6 @@ namespace {
 constexpr int FEW_THREADS = 256, FEW_WAVES = FEW_THREADS / 64;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // N elements of T as loaded: 4, 8 or 16 bytes at a time.
 template <typename T, int N>
