@@ -529,7 +529,8 @@ const float *pk_engine_rope(pk_engine *e, int *n_pos);
  * [n_tokens][n_heads] the logarithm of the softmax's denominator, sink
  * included. Rows of no prompt are left as they were. Scores, softmax and sums
  * are fp32; with 16-bit types the probabilities are rounded to that type for the
- * product with V, with PK_T_F32 products are exact to about 2^-23. Row t of q,
+ * product with V (fp16: scaled up, so that the step is never more than 2^-31 of
+ * the row's largest), with PK_T_F32 products are exact to about 2^-23. Row t of q,
  * k, v and out starts t * stride elements behind the pointer, its heads side by
  * side; pointers 16-byte aligned, strides multiples of 8 up to 2^26, head_dim a
  * multiple of 16 up to 128; out may not overlap the inputs. max_len: a bound on

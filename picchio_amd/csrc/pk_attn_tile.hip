@@ -208,6 +208,9 @@ __global__ __launch_bounds__(64 * WV, tile_simd(HDP, QP)) void k_attn_tile(pk_at
     constexpr int CPR = HDP / 8, KPW = 64 / CPR, PW = WV * KPW > KT ? KT / KPW : WV, RPP = PW * KPW, NP = KT / RPP, ROWB = HDP * 2;
     constexpr bool PLANES = QP > 1;
     constexpr int BUFS = tile_bufs(WV, QP);
+    // fp16 probabilities are scaled by 2^7 (at most 2^15 with what the reference lags), so that
+    // those down to 2^-21 of the largest are no subnormals
+    constexpr float SHIFT = __is_same(T, pk_f16) ? 7.0f : 0.0f;
     constexpr uint64_t ALL = KT == 64 ? ~0ull : (1ull << KT) - 1;
     typedef typename regs<T, 8>::type t8;
     typedef typename regs<C, 8>::type c8;
@@ -482,7 +485,7 @@ __global__ __launch_bounds__(64 * WV, tile_simd(HDP, QP)) void k_attn_tile(pk_at
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][b][i]);
             const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-            top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * scale2;
+            top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * scale2 - SHIFT;
             // the reference only moves when a score is 2^8 above it: what lies between makes
             // sums and probabilities no less exact, and most tiles need no rescaling
             if (__any(top > mx + 8.0f)) {

@@ -122,6 +122,26 @@ def test_packed_lowest_and_equal_scores(eng):
         assert torch.isfinite(p.out).all() and torch.isfinite(p.lse).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_small_probabilities(eng, dtype):
+    """One key far above all others, without a value of its own: the rest, each of a
+    probability around 1.03 * 2^-20 and large values, make up the result."""
+    gen = torch.Generator(device="cuda").manual_seed(22)
+    up = (20 - math.log2(1.03)) * math.log(2.0)
+    p = Packed(gen, [1800, 200], 8, 2, 64, dtype)
+    g = Paged(gen, [50, 1], [1900, 1700], 8, 2, 64, dtype, dtype, 16)
+    for x in (p, g):
+        x.q.fill_(1.0)
+    for k, v in [(p.k[:1800], p.v[:1800]), (p.k[1800:], p.v[1800:])] + list(zip(g.k, g.v)):
+        k.zero_()
+        k[0] = up / 8                                              # (64 elements, scale 1 / 8)
+        v *= 1024.0
+        v[0] = 0.0
+    g.fill()
+    p.run(eng), g.run(eng)
+    p.verify(what="packed"), g.verify(what="paged")
+
+
 def test_packed_bounds_of_starts(eng):
     """max_len cuts rows; starts beyond the rows or not ascending stay in bounds."""
     gen = torch.Generator(device="cuda").manual_seed(5)
